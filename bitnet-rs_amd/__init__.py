@@ -668,6 +668,22 @@ class HipLib:
     def gqa_prefill_last_groups(self) -> int:
         return int(self.c.bitnet_hip_gqa_prefill_last_groups())
 
+    def kv8_rows_dev(self, a: "Gqa", k_scale, v_scale, rows, ld: int, rows_f32: bool, pos, n: int, q=None, ldq: int = 0, stream: int = 0) -> None:
+        self._call("kv8_rows_dev", C.byref(a), _ptr(k_scale), _ptr(v_scale), _ptr(rows), _sz(ld), C.c_int(rows_f32), _ptr(pos), _sz(n), _optr(q), _sz(ldq), _vp(stream))
+
+    def kv8_read_dev(self, a: "Gqa", k_scale, v_scale, first: int, n: int, keys, values, f32: bool, stream: int = 0) -> None:
+        self._call("kv8_read_dev", C.byref(a), _ptr(k_scale), _ptr(v_scale), _sz(first), _sz(n), _optr(keys), _optr(values), C.c_int(f32), _vp(stream))
+
+    def kv8_step_dev(self, a: "Gqa", k_scale, v_scale, row, pos, scratch, stream: int = 0) -> None:
+        self._call("kv8_step_dev", C.byref(a), _ptr(k_scale), _ptr(v_scale), _ptr(row), _ptr(pos), _ptr(scratch), _vp(stream))
+
+    def kv8_prefill_scratch_bytes(self, a: "Gqa", n_ctx: int, nq: int) -> int:
+        self.c.bitnet_hip_kv8_prefill_scratch_bytes.restype = _sz
+        return int(self.c.bitnet_hip_kv8_prefill_scratch_bytes(C.byref(a), _sz(n_ctx), _sz(nq)))
+
+    def kv8_prefill_dev(self, a: "Gqa", k_scale, v_scale, q, ldq: int, n_ctx: int, nq: int, out, ldo: int, scratch=None, scratch_bytes: int = 0, stream: int = 0) -> None:
+        self._call("kv8_prefill_dev", C.byref(a), _ptr(k_scale), _ptr(v_scale), _ptr(q), _sz(ldq), _sz(n_ctx), _sz(nq), _ptr(out), _sz(ldo), _optr(scratch), _sz(scratch_bytes), _vp(stream))
+
     def delta_step_dev(self, d: "Delta", row, ba, pos, out, stream: int = 0) -> None:
         self._call("delta_step_dev", C.byref(d), _ptr(row), _ptr(ba), _ptr(pos), _ptr(out), _vp(stream))
 

@@ -211,6 +211,74 @@ int bitnet_hip_gqa_prefill_scratch_dev(const bitnet_hip_gqa *a, const uint16_t *
     BH_GUARD_END
 }
 
+// ---- attention over caches of 8 bits ------------------------------------------------------------------------------------
+static int check_kv8(const bitnet_hip_gqa *a, const float *k_scale, const float *v_scale) {
+    if (int rc = check_gqa(a)) return rc;
+    if (!gqa_supported((int)a->dimp, (int)a->vdimp)) return set_error(BITNET_HIP_ERR_UNSUPPORTED, "kv8: head of %zu / %zu columns", a->dimp, a->vdimp);
+    BH_REQUIRE(k_scale && v_scale && (((uintptr_t)a->kcache | (uintptr_t)a->vcache | (uintptr_t)k_scale | (uintptr_t)v_scale) & 15) == 0, "kv8: caches and scales on 16 bytes");
+    return 0;
+}
+static Kv8 kv8_of(const bitnet_hip_gqa *a, const float *k_scale, const float *v_scale) {
+    Kv8 c;
+    c.g = *a, c.k_scale = const_cast<float *>(k_scale), c.v_scale = const_cast<float *>(v_scale);
+    return c;
+}
+
+int bitnet_hip_kv8_rows_dev(const bitnet_hip_gqa *a, float *k_scale, float *v_scale, void *rows, size_t ld, int rows_f32, const int32_t *pos, size_t n, void *q, size_t ldq, void *stream) {
+    BH_GUARD_BEGIN
+    if (int rc = check_kv8(a, k_scale, v_scale)) return rc;
+    if (!q) ldq = ld;
+    BH_REQUIRE((q || a->taps == 0) && (!q || q != rows) && ldq >= a->heads * a->maps * a->dimp, "kv8_rows: bad place of the queries");
+    BH_REQUIRE(rows && pos && n > 0 && n <= a->capacity && ld >= gqa_row(a), "kv8_rows: bad arguments");
+    BH_REQUIRE((a->heads + a->kv_heads) * a->maps + a->kv_heads < 65536, "kv8_rows: too many heads");
+    BH_CHECK_DIMS(n, ld);
+    BH_CHECK_DIMS(n, ldq);
+    BH_HIP_TRY(launch_kv8_rows(kv8_of(a, k_scale, v_scale), rows, ld, rows_f32, pos, (int)n, q ? q : rows, ldq, (hipStream_t)stream));
+    return BITNET_HIP_OK;
+    BH_GUARD_END
+}
+
+int bitnet_hip_kv8_read_dev(const bitnet_hip_gqa *a, const float *k_scale, const float *v_scale, size_t first, size_t n, void *keys, void *values, int f32, void *stream) {
+    BH_GUARD_BEGIN
+    if (int rc = check_kv8(a, k_scale, v_scale)) return rc;
+    BH_REQUIRE((keys || values) && n > 0 && n <= a->capacity && first <= a->capacity - n && (((uintptr_t)keys | (uintptr_t)values) & 15) == 0 && a->kv_heads * (a->maps + 1) < 65536,
+               "kv8_read: bad arguments");
+    BH_HIP_TRY(launch_kv8_read(kv8_of(a, k_scale, v_scale), (int)first, (int)n, keys, values, f32, (hipStream_t)stream));
+    return BITNET_HIP_OK;
+    BH_GUARD_END
+}
+
+int bitnet_hip_kv8_step_dev(const bitnet_hip_gqa *a, float *k_scale, float *v_scale, const float *row, const int32_t *pos, float *scratch, void *stream) {
+    BH_GUARD_BEGIN
+    if (int rc = check_kv8(a, k_scale, v_scale)) return rc;
+    BH_REQUIRE(row && pos && scratch && (uintptr_t)scratch % 16 == 0, "kv8_step: bad arguments");
+    GqaStep s;
+    s.row = row, s.pos = pos, s.scratch = scratch;
+    BH_HIP_TRY(launch_kv8_step(kv8_of(a, k_scale, v_scale), s, (hipStream_t)stream));
+    return BITNET_HIP_OK;
+    BH_GUARD_END
+}
+
+size_t bitnet_hip_kv8_prefill_scratch_bytes(const bitnet_hip_gqa *a, size_t n_ctx, size_t nq) {
+    if (!a || check_gqa(a) != 0 || nq == 0 || nq > n_ctx || n_ctx > a->capacity || !gqa_supported((int)a->dimp, (int)a->vdimp)) return 0;
+    return kv8_prefill_floats(*a, (int)n_ctx, (int)nq) * sizeof(float);
+}
+
+int bitnet_hip_kv8_prefill_dev(const bitnet_hip_gqa *a, const float *k_scale, const float *v_scale, const uint16_t *q, size_t ldq, size_t n_ctx, size_t nq, uint16_t *out, size_t ldo,
+                               float *scratch, size_t scratch_bytes, void *stream) {
+    BH_GUARD_BEGIN
+    if (int rc = check_kv8(a, k_scale, v_scale)) return rc;
+    BH_REQUIRE(q && out && nq > 0 && nq <= n_ctx && n_ctx <= a->capacity && ldq % 8 == 0 && ldq >= a->heads * a->maps * a->dimp && ldo % 4 == 0 && ldo >= a->heads * a->vdimp &&
+                   (uintptr_t)q % 16 == 0 && (uintptr_t)out % 8 == 0,
+               "kv8_prefill: bad arguments");
+    BH_CHECK_DIMS(nq, ldq);
+    const size_t bytes = scratch ? kv8_prefill_floats(*a, (int)n_ctx, (int)nq) * sizeof(float) : 0;
+    BH_REQUIRE(bytes == 0 || ((uintptr_t)scratch % 16 == 0 && scratch_bytes >= bytes), "kv8_prefill: scratch of %zu bytes, %zu needed", scratch_bytes, bytes);
+    BH_HIP_TRY(launch_kv8_prefill(kv8_of(a, k_scale, v_scale), q, ldq, (int)n_ctx, (int)nq, out, ldo, bytes ? scratch : nullptr, (hipStream_t)stream));
+    return BITNET_HIP_OK;
+    BH_GUARD_END
+}
+
 // ---- gated delta rule -------------------------------------------------------------------------------------------------
 int bitnet_hip_delta_supported(size_t dimp, size_t vdimp) { return dimp <= 65536 && vdimp <= 65536 && delta_supported((int)dimp, (int)vdimp) ? 1 : 0; }
 int bitnet_hip_delta_chunked_supported(size_t dimp, size_t vdimp) { return dimp <= 65536 && vdimp <= 65536 && delta_chunked_supported((int)dimp, (int)vdimp) ? 1 : 0; }

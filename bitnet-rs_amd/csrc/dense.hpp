@@ -261,6 +261,18 @@ hipError_t launch_gqa_project(const GqaOut &a, hipStream_t s);
 extern thread_local int g_last_gqa_groups;  // groups of four waves per workgroup of launch_gqa_prefill's last launch on this thread
 size_t gqa_prefill_floats(const Gqa &g, int n_ctx, int nq);
 hipError_t launch_gqa_prefill(const Gqa &g, const uint16_t *q, size_t ldq, int n_ctx, int nq, uint16_t *out, size_t ldo, float *records, hipStream_t s);
+// the outputs, maxima and sums that a prompt's launch leaves of `parts` stretches of keys -> its outputs
+hipError_t launch_gqa_merge_parts(const Gqa &g, const float *records, int parts, int nq, uint16_t *out, size_t ldo, hipStream_t s);
+// caches of 8 bits (kcache, vcache: int8), a scale per head, map and position
+struct Kv8 {
+    Gqa g;
+    float *k_scale = nullptr, *v_scale = nullptr;  // [kv_heads][maps][capacity], [kv_heads][capacity]
+};
+hipError_t launch_kv8_rows(const Kv8 &c, const void *rows, size_t ld, int rows_f32, const int *pos, int n, void *q, size_t ldq, hipStream_t s);
+hipError_t launch_kv8_read(const Kv8 &c, int first, int n, void *keys, void *values, int f32, hipStream_t s);
+hipError_t launch_kv8_step(const Kv8 &c, const GqaStep &a, hipStream_t s);
+size_t kv8_prefill_floats(const Gqa &g, int n_ctx, int nq);
+hipError_t launch_kv8_prefill(const Kv8 &c, const uint16_t *q, size_t ldq, int n_ctx, int nq, uint16_t *out, size_t ldo, float *records, hipStream_t s);
 bool delta_supported(int dimp, int vdimp);
 bool delta_chunked_supported(int dimp, int vdimp);
 size_t delta_workspace_bytes(size_t n, size_t heads, size_t dimp, size_t vdimp);

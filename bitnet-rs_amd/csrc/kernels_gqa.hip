@@ -11,76 +11,9 @@
 //   k_gqa_merge    records of the decode forms -> output
 // Scores, maxima, sums and weights are f32; a weight (and the decode step's query) enters the matrix cores as a (high, low) pair of bf16 values.
 // Scores are kept in base 2: the score times log2(e).
-#include <algorithm>
-#include <type_traits>
-
-#include "dense.hpp"
+#include "gqa.hpp"
 
 namespace bitnet_hip {
-
-constexpr float kLog2e = 1.44269504088896f;
-
-// the first key a query at this position sees
-__host__ __device__ __forceinline__ int gqa_first(const Gqa &p, int pos) {
-    const int first = p.chunk ? pos - (int)((unsigned)pos % (unsigned)p.chunk) : 0;
-    return p.window && pos - (int)p.window + 1 > first ? pos - (int)p.window + 1 : first;
-}
-
-// The records of a query at `pos`: tiles of keys from `base` (the tile that holds its first key) on, `per` tiles each.
-struct GqaRange {
-    int first, base, per, used;
-};
-__device__ __forceinline__ GqaRange gqa_range(const Gqa &p, int pos) {
-    GqaRange r;
-    r.first = gqa_first(p, pos);
-    r.base = r.first & ~(kGqaTile - 1);
-    const int tiles = (pos + 1 - r.base + kGqaTile - 1) / kGqaTile;
-    r.per = (tiles + kGqaSplits - 1) / kGqaSplits;
-    r.used = (tiles + r.per - 1) / r.per;
-    return r;
-}
-// records a launch has to provide for
-static int gqa_records(const Gqa &g) {
-    size_t keys = g.capacity;
-    if (g.chunk && g.chunk + kGqaTile < keys) keys = g.chunk + kGqaTile;  // (a chunk may start inside a tile)
-    if (g.window && g.window + kGqaTile < keys) keys = g.window + kGqaTile;
-    return (int)min((size_t)kGqaSplits, (keys + kGqaTile - 1) / kGqaTile);
-}
-
-// element i of a head at a position, v being its own and the lane's neighbour holding the other element of the pair; cs, sn: the tables' row
-__device__ __forceinline__ float turn_neighbours(float v, int i, const float *cs, const float *sn, int dims) {
-    const float o = dpp<0xb1>(v);  // quad_perm [1,0,3,2]
-    if (i >= dims) return v;
-    const float c = cs[i >> 1], s = sn[i >> 1];
-    return (i & 1) ? v * c + o * s : v * c - o * s;
-}
-// what a head's gate (or that of a column of it) is the sigmoid of
-__device__ __forceinline__ float gate_logit(const Gqa &p, int row, int h, int column) {
-    const size_t i = (size_t)row * p.ldgate + (p.gate_columns ? (size_t)h * p.vdimp + column : (size_t)h);
-    return p.gate_f32 ? ((const float *)p.gate)[i] : bf2f(((const uint16_t *)p.gate)[i]);
-}
-// a head's distance penalty: what is taken off the natural score is weight * log2(1 + rate * distance)
-struct FarPenalty {
-    float weight, rate;
-};
-__device__ __forceinline__ FarPenalty far_penalty(const Gqa &p, int h) {
-    FarPenalty f{0.f, 0.f};
-    if (p.far_weight) f.weight = p.far_weight[h] * 0.69314718055994531f, f.rate = p.far_rate[h];
-    return f;
-}
-__device__ __forceinline__ float nearer(float score, const FarPenalty &f, int distance) { return fmaf(-f.weight, __log2f(fmaf(f.rate, (float)distance, 1.0f)), score); }
-// columns of a row of projections that a convolution covers
-__host__ __device__ __forceinline__ int gqa_channels(const Gqa &p) {
-    if (p.queries_only) return (int)(p.heads * p.maps * p.dimp);
-    return (int)((p.heads + p.kv_heads) * p.maps * p.dimp + (p.values_are_keys ? 0 : p.kv_heads * p.vdimp));
-}
-// column c of the row of projections t (negative: an earlier portion's; zero ahead of the sequence)
-template <class TR>
-__device__ __forceinline__ float raw_value(const Gqa &p, const TR *rows, size_t ld, int pos0, int t, int c, int channels) {
-    if (t >= 0) return ld_act(rows + (size_t)t * ld, c);
-    const int at = pos0 + t;
-    return at >= 0 ? p.ring[(size_t)(at % (int)p.taps) * channels + c] : 0.f;
-}
 
 size_t gqa_scratch_floats(size_t heads, size_t maps, size_t vdimp, size_t nq) { return nq * heads * maps * kGqaSplits * (kGqaRecHead + vdimp); }
 bool gqa_supported(int dimp, int vdimp) { return dimp <= 256 && vdimp <= 256; }
@@ -88,108 +21,6 @@ bool gqa_supported(int dimp, int vdimp) { return dimp <= 256 && vdimp <= 256; }
 // ---- rows of projections ----------------------------------------------------------------------------------------------
 // blockIdx.y: query heads x maps, key heads x maps (sixteen tokens per workgroup, four per wave), then value heads in groups of 32 columns (64
 // tokens, every fourth workgroup).
-constexpr int kRowTokens = 16, kRowCols = 32;
-
-// Four tokens of a query or key head of up to 128 NJ columns: a lane holds neighbouring elements, so that a pair turns within it.  TAPS: those of the convolution
-// (0: none, -1: any number).
-template <class TR, class TC, int NJ, int TAPS>
-__device__ __forceinline__ void head_rows(const Gqa &p, const TR *rows, size_t ld, int pos0, int t0, int n, int y, bool key, TC *cache, TR *queries, size_t ldq) {
-    constexpr int U = kRowTokens / 4;
-    constexpr bool CONV = TAPS != 0;
-    const int lane = threadIdx.x & 63, dim = (int)p.dim, dimp = (int)p.dimp, turned = (int)p.rot_dims, half = turned >> 1;
-    const float *w = key ? p.k_weight : p.q_weight;
-    float v[U][NJ][2], cs[U][NJ], sn[U][NJ], factor[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const int t = min(t0 + u, n - 1);
-        const TR *row = rows + (size_t)t * ld + (size_t)y * dimp;
-        factor[u] = key ? 1.0f : p.q_factor[pos0 + t];
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-            const int i = min(2 * lane + 128 * j, dimp - 2);
-            if (CONV)
-                v[u][j][0] = v[u][j][1] = 0.f;
-            else
-                v[u][j][0] = ld_act(row, i), v[u][j][1] = ld_act(row, i + 1);
-            cs[u][j] = 1.0f, sn[u][j] = 0.f;
-            if (turned && 2 * lane + 128 * j < turned) {
-                const size_t at = (size_t)(pos0 + t) * half + lane + 64 * j;
-                cs[u][j] = p.rope_cos[at], sn[u][j] = p.rope_sin[at];
-            }
-        }
-    }
-    if (TAPS > 0) {  // the tokens and those ahead of them once, in registers
-        constexpr int T = TAPS > 0 ? TAPS : 1;
-        const int channels = gqa_channels(p);
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-            const int c = y * dimp + min(2 * lane + 128 * j, dimp - 2);
-            float f[T][2], raw[U + T - 1][2];
-#pragma unroll
-            for (int k = 0; k < T; ++k) f[k][0] = p.conv[(size_t)k * channels + c], f[k][1] = p.conv[(size_t)k * channels + c + 1];
-            if (t0 >= T - 1) {
-#pragma unroll
-                for (int k = 0; k < U + T - 1; ++k) {
-                    const TR *row = rows + (size_t)min(t0 - (T - 1) + k, n - 1) * ld;
-                    raw[k][0] = ld_act(row, c), raw[k][1] = ld_act(row, c + 1);
-                }
-            } else {
-#pragma unroll
-                for (int k = 0; k < U + T - 1; ++k) {
-                    const int t = min(t0 - (T - 1) + k, n - 1);
-                    raw[k][0] = raw_value(p, rows, ld, pos0, t, c, channels), raw[k][1] = raw_value(p, rows, ld, pos0, t, c + 1, channels);
-                }
-            }
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-#pragma unroll
-                for (int k = 0; k < T; ++k) v[u][j][0] += f[k][0] * raw[u + k][0], v[u][j][1] += f[k][1] * raw[u + k][1];
-        }
-    } else if (CONV) {
-        const int taps = (int)p.taps, channels = gqa_channels(p);
-        for (int k = 0; k < taps; ++k)
-#pragma unroll
-            for (int j = 0; j < NJ; ++j) {
-                const int c = y * dimp + min(2 * lane + 128 * j, dimp - 2);
-                const float f0 = p.conv[(size_t)k * channels + c], f1 = p.conv[(size_t)k * channels + c + 1];
-#pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    const int t = min(t0 + u, n - 1) - (taps - 1) + k;
-                    v[u][j][0] += f0 * raw_value(p, rows, ld, pos0, t, c, channels), v[u][j][1] += f1 * raw_value(p, rows, ld, pos0, t, c + 1, channels);
-                }
-            }
-    }
-    float wv[NJ][2];
-#pragma unroll
-    for (int j = 0; j < NJ; ++j)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) wv[j][e] = w && 2 * lane + 128 * j + e < dim ? w[2 * lane + 128 * j + e] : 1.0f;  // (padding columns hold zeros)
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-        if (w || p.unit_norm) {
-            float ss = 0.f;
-#pragma unroll
-            for (int j = 0; j < NJ; ++j) ss += 2 * lane + 128 * j < dimp ? v[u][j][0] * v[u][j][0] + v[u][j][1] * v[u][j][1] : 0.f;
-            factor[u] *= 1.0f / sqrtf(wave_sum(ss) / (float)dim + p.eps);
-        }
-        if (t0 + u >= n) continue;
-        TR *row = queries + (size_t)(t0 + u) * ldq + (size_t)y * dimp;
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-            const int i = 2 * lane + 128 * j;
-            if (i >= dimp) continue;
-            const float a = v[u][j][0] * factor[u] * wv[j][0], b = v[u][j][1] * factor[u] * wv[j][1];
-            const float x = a * cs[u][j] - b * sn[u][j], z = b * cs[u][j] + a * sn[u][j];
-            if (key) {
-                TC *dst = cache + (size_t)(pos0 + t0 + u) * dimp;
-                st_act(dst, i, x), st_act(dst, i + 1, z);
-            } else {
-                st_act(row, i, x), st_act(row, i + 1, z);
-            }
-        }
-    }
-}
-
 // TAPS (as head_rows): every column passes a convolution over time first, and the queries go to a place of their own
 template <class TR, class TC, int NJ, int TAPS>
 __global__ __launch_bounds__(256) void k_gqa_rows(Gqa p, const TR *rows, size_t ld, const int *pos_ptr, int n, TR *queries, size_t ldq) {
@@ -1236,23 +1067,6 @@ __global__ __launch_bounds__(256 * G, NV > 8 || NK > 4 ? 1 : 2) void k_gqa_prefi
 
 thread_local int g_last_gqa_groups;
 
-// Two groups fill a CU, and halve its walks; of one group two workgroups fit.  They pay while the launch is as long as its longest walk: with four tiles or more in it, a CU's
-// share of all tiles not much above it, and no second round behind walks that are all long (the shortest walk of the first round and the longest of the second one in turn).
-// Heads count as a multiple of eight, as the launch deals them to the XCDs (20 heads take what 24 do).  us with two / with one: 24 heads, 2600 tokens
-// 80 / 90 (share / walk 1.05), 32 heads, 2048 63 / 75 (1.06), 40 heads, 1664 63 / 62 (1.09), 24 heads, 3000 105 / 105 (1.19), 3328 124 / 121 (1.27), 4096 173 / 153 (1.55); two maps,
-// 24 heads, 1280 39 / 44, 1531 57 / 53, 2048 88 / 75; five tiles 13.1 / 13.9, four 13.0 / 12.4.
-static bool two_groups(const Gqa &g, int rows, int n_ctx, int nq) {
-    const int at_once = 256, pos0 = n_ctx - nq, heads = ((int)g.heads + 7) / 8 * 8, blocks = (nq + rows - 1) / rows, all_tiles = (n_ctx + 63) / 64;
-    long longest = 0, total = 0, second = 0;
-    for (int qb = blocks - 1, done = 0; qb >= 0 && total <= 2l * at_once * all_tiles; --qb, done += heads) {
-        const int q0 = qb * rows, tiles = (std::min(n_ctx, pos0 + q0 + rows) + 63) / 64 - (gqa_first(g, pos0 + q0) >> 6);
-        longest = std::max<long>(longest, tiles), total += (long)heads * tiles;
-        for (int i : {at_once - 1, at_once})
-            if ((long)heads * blocks > at_once && done <= i && i < done + heads) second += tiles;
-    }
-    return longest >= 4 && 16 * total <= 17 * at_once * longest && 10 * second <= 11 * longest;
-}
-
 // The records of a query's head (gridDim.y of the launch above, one behind the other for every map) -> its output: a wave each, vdimp / 4 lanes of four columns, as many groups of them as fit a wave
 // sharing the records.
 template <int MAPS>
@@ -1296,19 +1110,11 @@ __global__ __launch_bounds__(256) void k_gqa_merge_parts(Gqa p, const float *rec
     if (grp == 0) *reinterpret_cast<bf16x4 *>(out + (size_t)qi * ldo + (size_t)h * vdimp + c) = bf16x4{(__bf16)q.x, (__bf16)q.y, (__bf16)q.z, (__bf16)q.w};
 }
 
-// Few queries behind many keys: a launch whose blocks leave CUs without a workgroup lasts as long as its longest walk, so a block's tiles are cut into stretches, of two tiles (a step of two
-// groups) at least and no more of them than there are CUs for (heads count as a multiple of eight, as the launch deals them to the XCDs: 12 heads in 21 stretches take 32 us where 15 take 24).
-// A step of a walk that is saved is worth 2.7 us (7 of one group); the launch that puts the records together costs 5 and 0.7 ns for each query's head, 1.4 for each of a head's two maps.
-// us without / with, heads, keys, queries: 12, 2090, 90 51 / 18; 24, 2090, 90 52 / 22; 12, 600, 20 18.3 / 11.1; 12, 1000, 200 28.7 / 18.9; 12, 450, 130 17.7 / 14.5; 12, 8000, 30 168 / 27;
-// 24 of two maps, 2090, 90 49 / 28; 2 of 256 columns, 2000, 50 131 / 22; 8, 2000, 2000 50 / 40.  What stays whole: 12, 400, 400 15.9 / 18.1; 16, 512, 512 18.6 / 21.2; 24 of two maps,
-// 600, 100 18.3 / 20.6; 12, 100, 3 8.4.
-static int gqa_prefill_parts(const Gqa &g, int n_ctx, int nq) {
-    const int rows = g.maps == 2 ? 64 : 128, blocks = (nq + rows - 1) / rows, heads = ((int)g.heads + 7) / 8 * 8;
-    const int tiles = (n_ctx + 63) / 64 - (gqa_first(g, n_ctx - nq + (blocks - 1) * rows) >> 6), most = std::min<long>(256 / ((long)heads * blocks), 32);
-    if (most < 2) return 1;
-    const int each = ((tiles + most - 1) / most + 1) & ~1, saved = (tiles + 1) / 2 - each / 2;
-    return 2.7 * saved > 5.0 + (g.maps == 2 ? 1.4e-3 : 7e-4) * (double)nq * (double)(g.heads * g.maps) ? (tiles + each - 1) / each : 1;
+hipError_t launch_gqa_merge_parts(const Gqa &g, const float *records, int parts, int nq, uint16_t *out, size_t ldo, hipStream_t s) {
+    hipLaunchKernelGGL(g.maps == 2 ? k_gqa_merge_parts<2> : k_gqa_merge_parts<1>, dim3((nq * (int)g.heads + 3) / 4), dim3(256), 0, s, g, records, parts, nq, out, ldo);
+    return hipGetLastError();
 }
+
 size_t gqa_prefill_floats(const Gqa &g, int n_ctx, int nq) {
     const int parts = gqa_prefill_parts(g, n_ctx, nq);
     return parts > 1 ? (size_t)nq * g.heads * g.maps * parts * (kGqaRecHead + g.vdimp) : 0;
@@ -1330,8 +1136,7 @@ static hipError_t gqa_prefill_go(const Gqa &g, const uint16_t *q, size_t ldq, in
     hipLaunchKernelGGL(fn, dim3(8 * ((g.heads + 7) / 8) * n_qb, parts), dim3(256 * G), lds, s, g, q, ldq, n_ctx, nq, out, ldo, n_qb, parts > 1 ? records : nullptr);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || parts == 1) return e;
-    hipLaunchKernelGGL(g.maps == 2 ? k_gqa_merge_parts<2> : k_gqa_merge_parts<1>, dim3((nq * (int)g.heads + 3) / 4), dim3(256), 0, s, g, records, parts, nq, out, ldo);
-    return hipGetLastError();
+    return launch_gqa_merge_parts(g, records, parts, nq, out, ldo, s);
 }
 
 // records: gqa_prefill_floats(g, n_ctx, nq) of them, or none where a block's keys stay together

@@ -858,6 +858,24 @@ int bitnet_hip_gqa_prefill_scratch_dev(const bitnet_hip_gqa *attn, const uint16_
 /* Groups of four waves that shared a query block's keys in the calling thread's last launch of it: 2, or 1 (few keys, or enough workgroups to fill the chip); 0: none yet. */
 int bitnet_hip_gqa_prefill_last_groups(void);
 
+/* The same attention over caches of 8 bits.  A head's key (of one map) and a head's value at a position are whole numbers -127 .. 127 with one scale: a = the largest magnitude, scale =
+ * a / 127, number = value * (127 / a) to the nearest, ties to even; a < 1.5e-36 counts as zero (scale 0), a vector with a value that is not finite has a scale that is not a number, and
+ * outputs that weigh it are none either.  In the attention's description kcache is int8 [kv_heads][maps][capacity][dimp], vcache int8 [kv_heads][capacity / 32][vdimp / 32][16][4][2][8]:
+ * column c at position p in [p / 32][c / 32][c % 16][p % 32 / 8][c % 32 / 16][p % 8].  k_scale [kv_heads][maps][capacity], v_scale [kv_heads][capacity].  All four on 16 bytes; nothing has to
+ * be cleared first (what lies past the positions written is not used).  The cache is a function of the tokens, whether they came as portions or one by one, and every position can be
+ * written again.  Heads of up to 256 columns (bitnet_hip_gqa_supported; others are refused). */
+/* as gqa_rows */
+int bitnet_hip_kv8_rows_dev(const bitnet_hip_gqa *attn, float *k_scale_dev, float *v_scale_dev, void *rows_dev, size_t ld, int rows_f32, const int32_t *pos_dev, size_t n, void *q_dev,
+                            size_t ldq, void *stream);
+/* positions first .. first + n - 1 as bf16 or f32: keys [kv_heads][maps][n][dimp], values [kv_heads][n][vdimp], on 16 bytes (either one NULL: left out) */
+int bitnet_hip_kv8_read_dev(const bitnet_hip_gqa *attn, const float *k_scale_dev, const float *v_scale_dev, size_t first, size_t n, void *keys_dev, void *values_dev, int f32, void *stream);
+/* as gqa_step: the row is appended by the same launch (the attention sees it as the cache holds it), and the records are those that gqa_merge, gqa_out and gqa_project take */
+int bitnet_hip_kv8_step_dev(const bitnet_hip_gqa *attn, float *k_scale_dev, float *v_scale_dev, const float *row_dev, const int32_t *pos_dev, float *scratch_dev, void *stream);
+/* as gqa_prefill_scratch (scratch NULL: the keys stay together); q as kv8_rows leaves it, out bf16 */
+size_t bitnet_hip_kv8_prefill_scratch_bytes(const bitnet_hip_gqa *attn, size_t n_ctx, size_t nq);
+int bitnet_hip_kv8_prefill_dev(const bitnet_hip_gqa *attn, const float *k_scale_dev, const float *v_scale_dev, const uint16_t *q_dev, size_t ldq, size_t n_ctx, size_t nq, uint16_t *out_dev,
+                               size_t ldo, float *scratch_dev, size_t scratch_bytes, void *stream);
+
 /* Gated delta rule.  A row of projections is [q kv_heads * dimp | k kv_heads * dimp | v heads * vdimp | gate heads * vdimp], and apart from it
  * [b heads | a heads] f32; heads zero-padded to multiples of 32.  q, k, v pass a causal convolution of `taps` tokens per channel and
  * silu; q and k are divided by sqrt(sum of squares + unit_eps) per head, q multiplied by q_scale; head h uses q/k head

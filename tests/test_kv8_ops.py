@@ -1,0 +1,408 @@
+"""The attention over caches of 8 bits (include/bitnet_hip.h section 5: kv8_rows, kv8_read, kv8_step, kv8_prefill), one operator at a time through the C ABI and then together, against f64
+numpy (tests/kv8_util.py).
+
+Tolerances.  A number of the cache is off by half a step of its scale at most, and by what 32 bits lose ahead of it (1e-5 of the largest).  STEP: a step's chain is 32 bits wide (norm, factor
+and scale: four roundings of 2^-24 on a score, of magnitude up to ten here: 2.4e-6), queries have 23 bits of their largest element and weights 22: together under 5e-6 of a weight, errors of
+different weights independent; twice that is allowed.  PROMPT: a weight is an f16 (2^-12), a query 15 bits of its largest element (a few 2^-16 of a score of up to ten: 5e-4): 2^-10; and the
+output a bf16 (2^-9 at most).  Two maps: what their difference makes of either's error (kv8_util.Attention.want)."""
+import numpy as np
+import pytest
+
+from tests import kv8_util as kv
+from tests import stack_util as u
+
+pytestmark = pytest.mark.gpu
+STEP, PROMPT = 1e-5, (2.0 ** -10, 2.0 ** -9)
+f64 = np.float64
+
+
+def as_bf16(t):
+    import torch
+
+    return t.bfloat16().view(torch.int16)
+
+
+# heads, kv heads, dim, vdim, maps
+SHAPES = [(4, 2, 24, 40, 2), (6, 6, 128, 128, 2), (20, 1, 64, 100, 2), (8, 2, 96, 64, 1), (2, 1, 200, 256, 2), (5, 1, 40, 16, 1), (34, 2, 16, 24, 2), (8, 2, 128, 128, 1), (3, 3, 64, 64, 1),
+          (16, 2, 256, 160, 1)]
+# what else an attention can have, on heads that take it
+OPTIONS = [dict(rot=16), dict(rot=24, window=37), dict(chunk=50, sink=True, gate="heads", rot=8), dict(far=True, gate="columns", window=100), dict(keys_as_values=True, normed=False, sink=True),
+           dict(normed=False, far=True), dict(gate="columns")]
+
+
+# ---- writing ------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("f32", [True, False])
+@pytest.mark.parametrize("n0,n", [(0, 1), (31, 1), (5, 2), (31, 2), (0, 32), (7, 33), (17, 130), (64, 64), (3, 300)])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_written_bit_by_bit(hip, pkg, shape, n0, n, f32):
+    """keys and values without anything ahead of them: numbers and scales as the rule gives them, everything else as it was"""
+    t = kv.Attention(pkg, n0 + n, *shape, normed=False, f32=f32, fill=77, scale=5.0)
+    _, q = t.fill(hip, n0, n0 + n)
+    k, v, ks, vs = t.cache.host()
+    for got, scales, x in ((k, ks, t.k), (v, vs, t.v)):
+        numbers, scale = kv.numbers_of(x)
+        assert np.array_equal(got[..., n0:n0 + n, :], numbers[..., n0:n0 + n, :]) and np.array_equal(scales[..., n0:n0 + n], scale[..., n0:n0 + n])
+        assert (got[..., :n0, :] == 77).all() and (got[..., n0 + n:, :] == 77).all() and (scales[..., :n0] == 5).all() and (scales[..., n0 + n:] == 5).all()
+    got = u.host(q).reshape(n, -1, t.dimp)
+    assert u.rms_error(got[..., :t.dim], t.q[n0:]) < (1e-6 if f32 else 2.0 ** -8) and not got[..., t.dim:].any()
+
+
+@pytest.mark.parametrize("f32", [True, False])
+@pytest.mark.parametrize("options", [dict(), dict(rot=16), dict(taps=3), dict(taps=5, rot=24), dict(taps=1, keys_as_values=True), dict(keys_as_values=True, rot=4)])
+@pytest.mark.parametrize("shape", [(6, 2, 24, 24, 1), (4, 2, 128, 128, 1), (2, 1, 200, 200, 1), (4, 2, 64, 100, 2)])
+def test_written_behind_norms_and_convolutions(hip, pkg, shape, options, f32):
+    if shape[4] == 2 and options.get("keys_as_values"):
+        pytest.skip("two maps have values of their own")
+    t = kv.Attention(pkg, 210, *shape, f32=f32, **options)
+    for n0, n1 in ((0, 3), (3, 4), (4, 130), (130, 210)):
+        rows, q = t.fill(hip, n0, n1)
+        got = u.host(q).reshape(n1 - n0, -1, t.dimp)
+        assert u.rms_error(got[..., :t.dim], t.q[n0:n1]) < (3e-6 if f32 else 2.0 ** -8)
+        assert np.array_equal(u.host(rows), t.rows[n0:n1])
+    k, v, ks, vs = t.cache.host()
+    for got, scales, x in ((k, ks, t.k), (v, vs, t.v)):
+        got, scales = got[..., :210, :].astype(f64), scales[..., :210].astype(f64)
+        largest = np.abs(x).max(-1)
+        assert np.abs(scales * 127 / largest - 1).max() < 1e-5
+        assert (np.abs(got * scales[..., None] - x) <= scales[..., None] * 0.5 + 1e-5 * largest[..., None]).all()
+
+
+def test_queries_in_place_and_rows_of_odd_leading_dimension(hip, pkg):
+    t = kv.Attention(pkg, 40, 5, 1, 40, 16)
+    rows = np.full((40, t.ld + 3), 7, np.float32)
+    rows[:, :t.ld] = t.rows
+    d = u.dev_bf16(rows)
+    pos = u.dev(np.array([0], np.int32))
+    hip.kv8_rows_dev(t.attn, t.cache.ks, t.cache.vs, d, t.ld + 3, False, pos, 40)
+    got, nq = u.host(d), t.heads * t.dimp
+    assert np.array_equal(got[:, nq:], rows[:, nq:]) and u.rms_error(got[:, :nq].reshape(40, 5, -1)[..., :40], t.q) < 2.0 ** -8
+    before = t.cache.host()
+    t.fill(hip, 0, 40)
+    assert all(np.array_equal(a, b) for a, b in zip(before, t.cache.host()))
+
+
+def test_values_that_no_scale_fits(hip, pkg):
+    """zeros, tiny and huge numbers, infinities and NaN: zeros, numbers or no numbers, each position by itself"""
+    t = kv.Attention(pkg, 40, 2, 1, 64, 64, normed=False, f32=True, seed=3)
+    nq, nk = 2 * 64, 64
+    for i, x in enumerate((0.0, 1e-37, 1e-45, 1.4e-36, 1.6e-36, 1e30, 3e38, np.inf, -np.inf, np.nan)):
+        t.rows[i, nq:nq + 2 * nk] *= 0
+        t.rows[i, nq + 5] = t.rows[i, nq + nk + 60] = x
+        t.rows[i, nq + 6] = t.rows[i, nq + nk + 3] = 0 if not np.isfinite(x) else -x / 3
+    t.fill(hip, 0, 40)
+    k, v, ks, vs = t.cache.host()
+    for got, scales, first in ((k[0, 0], ks[0, 0], nq), (v[0], vs[0], nq + nk)):
+        numbers, scale = kv.numbers_of(t.rows[:, first:first + nk])
+        assert np.array_equal(got[:40], numbers) and np.array_equal(scales[:40], scale, equal_nan=True)
+        assert np.isnan(scales[7:10]).all() and (scales[:4] == 0).all() and (scales[4:7] > 0).all()
+
+
+@pytest.mark.parametrize("shape", SHAPES[:6])
+def test_portions_and_steps_write_the_same(hip, pkg, shape):
+    """the cache is a function of the tokens: at once, in portions, and one by one"""
+    n = 70
+    whole, cut, steps = (kv.Attention(pkg, n, *shape, f32=True, rot=8) for _ in range(3))
+    whole.fill(hip, 0, n)
+    for n0, n1 in ((0, 1), (1, 30), (30, 33), (33, 70)):
+        cut.fill(hip, n0, n1)
+    for i in range(n):
+        steps.step(hip, i)
+    a = whole.cache.host()
+    assert all(np.array_equal(x, y) for x, y in zip(a, cut.cache.host()))
+    for x, y, held in zip(a[2:], steps.cache.host()[2:], (whole.k, whole.v)):  # (a step sums a norm in another order)
+        assert np.allclose(x, y, rtol=1e-6, atol=0)
+    for x, y in zip(a[:2], steps.cache.host()[:2]):
+        assert np.abs(x.astype(int) - y).max() <= 1 and (x != y).mean() < 1e-3
+
+
+def test_a_position_written_again(hip, pkg):
+    t, other = (kv.Attention(pkg, 50, 4, 2, 24, 40, 2, seed=s) for s in (0, 1))
+    other.fill(hip, 0, 50)
+    t.attn.kcache, t.attn.vcache, cache, t.cache = other.cache.k.data_ptr(), other.cache.v.data_ptr(), t.cache, other.cache
+    t.fill(hip, 10, 37)
+    k, v, ks, vs = t.cache.host()
+    t.attn.kcache, t.attn.vcache, t.cache = cache.k.data_ptr(), cache.v.data_ptr(), cache
+    t.fill(hip, 10, 37)
+    assert all(np.array_equal(a[..., 10:37, :], b[..., 10:37, :]) for a, b in zip((k, v), t.cache.host()))
+    other.fill(hip, 10, 37)
+    again = other.cache.host()
+    fresh = kv.Attention(pkg, 50, 4, 2, 24, 40, 2, seed=1)
+    fresh.fill(hip, 0, 50)
+    assert all(np.array_equal(a, b) for a, b in zip(again, fresh.cache.host()))
+
+
+# ---- reading back -------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("f32", [True, False])
+@pytest.mark.parametrize("first,n", [(0, 1), (31, 1), (31, 2), (0, 384), (5, 300), (96, 33), (383, 1)])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_read_back(hip, pkg, shape, first, n, f32):
+    import torch
+
+    heads, g, dim, vdim, maps = shape
+    t = kv.Attention(pkg, 384, heads, g, dim, vdim, maps)
+    gen = torch.Generator(device="cuda").manual_seed(n)
+    c = t.cache
+    for x in (c.k, c.v):
+        x.copy_(torch.randint(-127, 128, x.shape, generator=gen, device="cuda", dtype=torch.int8))
+    for x in (c.ks, c.vs):
+        x.copy_(torch.rand(x.shape, generator=gen, device="cuda"))
+    new = torch.float32 if f32 else torch.bfloat16
+    keys, values = torch.full((g, maps, n, t.dimp), 3, dtype=new, device="cuda"), torch.full((g, n, t.vdimp), 3, dtype=new, device="cuda")
+    hip.kv8_read_dev(t.attn, c.ks, c.vs, first, n, keys, values, f32)
+    k, v, ks, vs = c.host()
+    for got, numbers, scale in ((keys, k, ks), (values, v, vs)):
+        want = numbers[..., first:first + n, :].astype(np.float32) * scale[..., first:first + n, None]
+        assert np.array_equal(got.float().cpu().numpy(), want if f32 else u.rounded(want))
+    for which in (0, 1):
+        a, b = torch.zeros_like(keys), torch.zeros_like(values)
+        hip.kv8_read_dev(t.attn, c.ks, c.vs, first, n, None if which else a, b if which else None, f32)
+        assert bool((a == (0 * keys if which else keys)).all()) and bool((b == (values if which else 0 * values)).all())
+
+
+# ---- steps --------------------------------------------------------------------------------------------------------------
+def stepped(hip, t, i):
+    if i:
+        t.fill(hip, 0, i)
+    before = [a.copy() for a in t.cache.host()]
+    out = t.step(hip, i)
+    t.check(out, t.want(t.q[i:i + 1], i), STEP)
+    for a, b in zip(before, t.cache.host()):  # nothing but the position
+        axis = b.ndim - 2 if a.dtype == np.int8 else b.ndim - 1
+        assert np.delete(a, i, axis).tobytes() == np.delete(b, i, axis).tobytes()  # (some are no numbers)
+    numbers, scale = kv.numbers_of(t.k[..., i, :])
+    assert np.allclose(t.cache.host()[2][..., i], scale, rtol=1e-5) and np.abs(t.cache.host()[0][..., i, :].astype(int) - numbers).max() <= 1
+    if t.maps == 2:  # (keys of another layer: one map)
+        return
+    kept = t.cache.host()
+    t.check(t.step(hip, i, queries_only=True), t.want(t.q[i:i + 1], i), STEP)
+    assert all(a.tobytes() == b.tobytes() for a, b in zip(kept, t.cache.host()))
+
+
+@pytest.mark.parametrize("n", [1, 2, 32, 33, 64, 65, 127, 128, 129, 257, 700])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_step(hip, pkg, shape, n):
+    """garbage behind the positions written, scales that are no numbers among it"""
+    stepped(hip, kv.Attention(pkg, n, *shape, fill=-128, scale=np.nan), n - 1)
+
+
+@pytest.mark.parametrize("options", OPTIONS)
+@pytest.mark.parametrize("n", [1, 33, 100, 129, 300])
+@pytest.mark.parametrize("shape", [(6, 2, 24, 24), (4, 4, 128, 128), (20, 1, 96, 96), (2, 1, 200, 200)])
+def test_step_with_everything_else(hip, pkg, shape, n, options):
+    stepped(hip, kv.Attention(pkg, n, *shape, fill=99, scale=np.inf, **options), n - 1)
+
+
+@pytest.mark.parametrize("n,window", [(17000, 0), (40000, 0), (40000, 700), (16513, 16384)])
+def test_step_behind_many_keys(hip, pkg, n, window):
+    """records of several tiles; sharp scores"""
+    t = kv.Attention(pkg, n, 3, 1, 64, 64, window=window, sharp=3.0)
+    t.fill(hip, 0, n - 1)
+    t.check(t.step(hip, n - 1), t.want(t.q[n - 1:], n - 1), STEP * 3)
+
+
+@pytest.mark.parametrize("spread", [1e-30, 1e-3, 1e3, 1e30])
+def test_values_of_very_different_size(hip, pkg, spread):
+    """scales grow and shrink by the token: what is large decides, whatever came ahead of it"""
+    for n in (40, 300):
+        t = kv.Attention(pkg, n, 4, 2, 64, 64, normed=False, f32=True)
+        at = 4 * t.dimp + 2 * t.dimp
+        t.rows[::7, at:at + 2 * t.vdimp] *= np.float32(spread)
+        t.convolved = t.rows[:, :t.channels].astype(f64)
+        t.fill(hip, 0, n - 1)
+        t.check(t.step(hip, n - 1), t.want(t.q[n - 1:], n - 1), STEP)
+        _, q = t.fill(hip, 0, n)
+        qb = as_bf16(q)
+        t.check(t.prompt(hip, qb, 0, n), t.want(u.host(qb).reshape(n, -1, t.dimp)[..., :t.dim], 0), *PROMPT)
+
+
+# ---- prompts ------------------------------------------------------------------------------------------------------------
+def prompted(hip, t, n0, n):
+    if n0:
+        t.fill(hip, 0, n0)
+    _, q = t.fill(hip, n0, n)
+    want = t.want(u.host(q).reshape(n - n0, -1, t.dimp)[..., :t.dim], n0)
+    outs = [t.prompt(hip, q, n0, n, split) for split in (True, False)]
+    for out in outs:
+        t.check(out, want, *PROMPT)
+
+
+@pytest.mark.parametrize("n,nq", [(1, 1), (2, 2), (63, 63), (65, 65), (128, 128), (129, 2), (200, 200), (333, 70), (600, 5)])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_prompt(hip, pkg, shape, n, nq):
+    prompted(hip, kv.Attention(pkg, n, *shape, fill=-128, scale=np.nan), n - nq, n)
+
+
+@pytest.mark.parametrize("options", OPTIONS)
+@pytest.mark.parametrize("n,nq", [(1, 1), (130, 130), (333, 40)])
+@pytest.mark.parametrize("shape", [(6, 2, 24, 24), (4, 4, 128, 128), (20, 1, 96, 96), (2, 1, 200, 200)])
+def test_prompt_with_everything_else(hip, pkg, shape, n, nq, options):
+    prompted(hip, kv.Attention(pkg, n, *shape, fill=99, scale=np.inf, **options), n - nq, n)
+
+
+@pytest.mark.parametrize("shape", [(8, 2, 128, 128, 1), (4, 1, 64, 128, 2), (9, 3, 64, 64, 1), (2, 1, 256, 256, 1)])
+@pytest.mark.parametrize("n,nq", [(1100, 1100), (2500, 40), (2500, 130)])
+def test_long_prompts(hip, pkg, shape, n, nq):
+    """one group and two, stretches and whole walks; a sample of the queries by definition"""
+    t = kv.Attention(pkg, n, *shape, rot=16, sharp=2.0)
+    if n > nq:
+        t.fill(hip, 0, n - nq)
+    _, q = t.fill(hip, n - nq, n)
+    some = np.unique(np.linspace(0, nq - 1, 23).astype(int))
+    held, qh = t.cache.held(), u.host(q).reshape(nq, -1, t.dimp)[..., :t.dim]
+    want = np.concatenate([t.want(qh[i:i + 1], n - nq + i, held) for i in some])
+    for split in (True, False):
+        t.check(u.dev_f32(u.host(t.prompt(hip, q, n - nq, n, split))[some]), want, *PROMPT)
+
+
+# ---- what must not spread -----------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("what", ["key", "value"])
+def test_a_token_without_numbers_reaches_who_sees_it(hip, pkg, what):
+    """a NaN in one token's key or value: earlier queries and those whose window has passed keep their outputs, the others have none"""
+    n, bad, window = 200, 70, 60
+    t = kv.Attention(pkg, n, 4, 2, 64, 64, window=window, f32=True)
+    clean = kv.Attention(pkg, n, 4, 2, 64, 64, window=window, f32=True)
+    at = 4 * t.dimp + (0 if what == "key" else 2 * t.dimp)
+    for a in (t, clean):  # (not the largest of its tile: what the others' weights are brought to stays the same)
+        a.rows[bad, 6 * t.dimp:8 * t.dimp] *= 0.01
+        a.convolved[bad, 6 * t.dimp:8 * t.dimp] *= 0.01
+    t.rows[bad, at + 3] = t.convolved[bad, at + 3] = np.nan  # (the first kv head's: heads 0 and 1)
+    outs = []
+    for a in (t, clean):
+        _, q = a.fill(hip, 0, n)
+        outs.append(u.host(a.prompt(hip, as_bf16(q), 0, n)).reshape(n, 4, 64))
+    sees = np.arange(n)
+    sees = (sees >= bad) & (sees < bad + window)
+    assert np.isnan(outs[0][sees][:, :2]).all()
+    assert np.array_equal(outs[0][~sees], outs[1][~sees]) and np.array_equal(outs[0][:, 2:], outs[1][:, 2:])
+    for i in (bad - 1, bad, bad + window - 1, bad + window, n - 1):
+        got, want = (u.host(a.step(hip, i)).reshape(4, 64) for a in (t, clean))
+        assert np.isnan(got[:2]).all() if sees[i] else np.array_equal(got, want)
+        assert np.array_equal(got[2:], want[2:])
+
+
+def test_queries_without_numbers(hip, pkg):
+    """a query that is not finite has no output, one of zeros weighs all keys alike, and no other query notices"""
+    n = 150
+    t = kv.Attention(pkg, n, 4, 2, 64, 64, normed=False, f32=True)
+    _, q = t.fill(hip, 0, n)
+    q[20, 64:128] = float("inf")
+    q[40, 3] = float("nan")
+    q[60] = 0
+    q = as_bf16(q)
+    got = u.host(t.prompt(hip, q, 0, n)).reshape(n, 4, 64)
+    assert np.isnan(got[20, 1]).all() and np.isnan(got[40, 0]).all()
+    got[20, 1] = got[40, 0] = 0
+    qh = u.host(q).reshape(n, 4, 64)
+    qh[20, 1] = qh[40, 0] = 0
+    want = t.want(qh, 0)
+    want[20, 1] = want[40, 0] = 0
+    t.check(u.dev_f32(got), want, *PROMPT)
+    mean = t.cache.held()[1][0, :61].mean(0)
+    assert u.rms_error(got[60, 0], mean) < sum(PROMPT)
+
+
+# ---- together -----------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("shape", [(20, 5, 128, 128, 1), (12, 3, 64, 128, 2), (6, 2, 96, 96, 1)])
+def test_a_sequence_as_it_is_used(hip, pkg, shape):
+    """two portions, then steps; the outputs against f64 over the cache and over keys and values that were never rounded, and the cache read back"""
+    import torch
+
+    n = 330
+    t = kv.Attention(pkg, n, *shape, rot=32, f32=False)
+    for n0, n1 in ((0, 130), (130, 300)):
+        _, q = t.fill(hip, n0, n1)
+        out = t.prompt(hip, q, n0, n1)
+        t.check(out, t.want(u.host(q).reshape(n1 - n0, -1, t.dimp)[..., :t.dim], n0), *PROMPT)
+    for i in range(300, n):
+        out = t.step(hip, i)
+        t.check(out, t.want(t.q[i:i + 1], i), STEP)
+        # A number is off by a step / sqrt(12), steps being independent: a score by |q| (a key's scale) / sqrt(12), which is what a weight is off by, and a value by its scale / sqrt(12).
+        # The output, a sum of values with independent errors, is off by both together, relative to the values; three times the largest of either is allowed.
+        _, _, ks, vs = t.cache.host()
+        off = 3 / np.sqrt(12) * (np.linalg.norm(t.q[i], axis=-1).max() * ks[..., :i + 1].max() + (vs[:, :i + 1] / np.sqrt((t.v[:, :i + 1] ** 2).mean(-1))).max())
+        t.check(out, t.want(t.q[i:i + 1], i, (t.k, t.v)), off)
+    keys, values = torch.zeros(shape[1], shape[4], n, t.dimp, device="cuda"), torch.zeros(shape[1], n, t.vdimp, device="cuda")
+    hip.kv8_read_dev(t.attn, t.cache.ks, t.cache.vs, 0, n, keys, values, True)
+    for got, x in ((keys, t.k), (values, t.v)):
+        assert (np.abs(got.cpu().numpy() - x) <= np.abs(x).max(-1, keepdims=True) * (0.5 / 127 + 1e-5)).all()
+
+
+def test_two_streams_and_a_graph(hip, pkg):
+    """a captured step and prompt, replayed at other positions among eager work on other streams, give what eager calls give; two captures with scratch of their own do not meet"""
+    import torch
+
+    n = 260
+    a, b = (kv.Attention(pkg, n, 8, 2, 128, 128, rot=64, f32=True, seed=s) for s in (0, 1))
+    side = torch.cuda.Stream()
+    held = []
+    for t in (a, b):
+        t.fill(hip, 0, n)
+        held.append([x.clone() for x in (t.cache.k, t.cache.v, t.cache.ks, t.cache.vs)])
+    positions = [200, 129, 64, 259, 0]
+    for t in (a, b):  # (as steps leave the positions)
+        for i in positions:
+            t.step(hip, i)
+    want = [[u.host(t.step(hip, i)).copy() for i in positions] for t in (a, b)]
+    graphs = []
+    for t in (a, b):
+        pos, row = u.dev(np.array([0], np.int32)), u.zeros_f32(t.ld)
+        scratch, out = u.zeros_f32(hip.gqa_scratch_bytes(8, 1, 128, 1) // 4), u.zeros_f32(1, 8 * 128)
+        q, prompt = u.zeros_bf16(n, 8 * 128), u.zeros_bf16(n, 8 * 128)
+        q.copy_(as_bf16(u.dev_f32(t.q.reshape(n, -1))))
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            s = torch.cuda.current_stream().cuda_stream
+            hip.kv8_step_dev(t.attn, t.cache.ks, t.cache.vs, row, pos, scratch, stream=s)
+            hip.gqa_merge_dev(t.attn, pos, 0, 1, scratch, out, 8 * 128, False, stream=s)
+            hip.kv8_prefill_dev(t.attn, t.cache.ks, t.cache.vs, q, q.shape[1], n, n, prompt, 8 * 128, stream=s)
+        graphs.append((graph, pos, row, out, q, prompt, scratch))  # (all of them live as long as the graph)
+    eager = [u.host(t.prompt(hip, g[4], 0, n, split=False)).copy() for t, g in zip((a, b), graphs)]
+    for k, i in enumerate(positions):
+        for t, (_, pos, row, *_) in zip((a, b), graphs):
+            pos.fill_(i)
+            row.copy_(u.dev_f32(t.rows[i]))
+        torch.cuda.synchronize()
+        graphs[0][0].replay()
+        with torch.cuda.stream(side):
+            graphs[1][0].replay()
+        torch.cuda.synchronize()
+        for w in range(2):
+            assert np.array_equal(u.host(graphs[w][3]), want[w][k]), (w, i)
+            assert np.array_equal(u.host(graphs[w][5]), eager[w]), (w, i)
+        t = (a, b)[k & 1]
+        u.host(t.step(hip, positions[k - 1]))
+    for t, before in zip((a, b), held):
+        t.fill(hip, 0, n)
+        assert all(bool((x == y).all()) for x, y in zip(before, (t.cache.k, t.cache.v, t.cache.ks, t.cache.vs)))
+
+
+def test_caches_past_two_gigabytes(hip, pkg):
+    """8 heads of 256 columns at a capacity of 1310720: offsets of the last head pass 32 bits"""
+    import torch
+
+    cap, kvh, heads = 1310720, 8, 8
+    base = cap - 700
+    small = kv.Attention(pkg, 640, heads, kvh, 256, 256, window=200, f32=True)
+    t = kv.Attention(pkg, 640, heads, kvh, 256, 256, window=200, f32=True)
+    big = kv.Cache(kvh, 1, cap, 256, 256)
+    factor = torch.zeros(cap, device="cuda")
+    factor[base:base + 640] = t.keep[2][:640]
+    t.attn.capacity, t.attn.kcache, t.attn.vcache, t.attn.q_factor = cap, big.k.data_ptr(), big.v.data_ptr(), factor.data_ptr()
+    rows, pos, q = t.put(t.rows), u.dev(np.array([base], np.int32)), u.zeros_f32(640, heads * 256)
+    hip.kv8_rows_dev(t.attn, big.ks, big.vs, rows, t.ld, True, pos, 640, q, q.shape[1])
+    _, qs = small.fill(hip, 0, 640)
+    assert bool((q == qs).all())
+    got, want = u.zeros_bf16(300, heads * 256), u.zeros_bf16(300, heads * 256)
+    hip.kv8_prefill_dev(t.attn, big.ks, big.vs, as_bf16(q)[340:].contiguous(), heads * 256, base + 640, 300, got, heads * 256)
+    hip.kv8_prefill_dev(small.attn, small.cache.ks, small.cache.vs, as_bf16(qs)[340:].contiguous(), heads * 256, 640, 300, want, heads * 256)
+    assert u.rms_error(u.host(got), u.host(want)) < sum(PROMPT)  # (tiles of keys begin elsewhere)
+    keys, values = torch.zeros(kvh, 1, 640, 256, device="cuda"), torch.zeros(kvh, 640, 256, device="cuda")
+    hip.kv8_read_dev(t.attn, big.ks, big.vs, base, 640, keys, values, True)
+    k, v = small.cache.held()
+    assert u.rms_error(keys.cpu().numpy(), k) < 1e-7 and u.rms_error(values.cpu().numpy(), v) < 1e-7
+    scratch, out = u.zeros_f32(hip.gqa_scratch_bytes(heads, 1, 256, 1) // 4), u.zeros_f32(1, heads * 256)
+    at = u.dev(np.array([base + 639], np.int32))
+    hip.kv8_step_dev(t.attn, big.ks, big.vs, u.dev_f32(t.rows[639]), at, scratch)
+    hip.gqa_merge_dev(t.attn, at, 0, 1, scratch, out, heads * 256, False)
+    assert u.rms_error(u.host(out), u.host(small.step(hip, 639))) < 2 * STEP

@@ -272,7 +272,8 @@ int bitnet_hip_kv8_prefill_dev(const bitnet_hip_gqa *a, const float *k_scale, co
                    (uintptr_t)q % 16 == 0 && (uintptr_t)out % 8 == 0,
                "kv8_prefill: bad arguments");
     BH_CHECK_DIMS(nq, ldq);
-    const size_t bytes = scratch ? kv8_prefill_floats(*a, (int)n_ctx, (int)nq) * sizeof(float) : 0;
+    const size_t bytes = scratch || kv8_prefill_wants_records(*a) ? kv8_prefill_floats(*a, (int)n_ctx, (int)nq) * sizeof(float) : 0;
+    BH_REQUIRE(bytes == 0 || scratch, "kv8_prefill: two maps of heads of more than 128 columns want scratch");
     BH_REQUIRE(bytes == 0 || ((uintptr_t)scratch % 16 == 0 && scratch_bytes >= bytes), "kv8_prefill: scratch of %zu bytes, %zu needed", scratch_bytes, bytes);
     BH_HIP_TRY(launch_kv8_prefill(kv8_of(a, k_scale, v_scale), q, ldq, (int)n_ctx, (int)nq, out, ldo, bytes ? scratch : nullptr, (hipStream_t)stream));
     return BITNET_HIP_OK;

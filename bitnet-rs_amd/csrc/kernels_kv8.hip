@@ -8,9 +8,9 @@
 //   k_kv8_read     positions back as bf16 or f32
 //   k_kv8_step     the decode step, records as k_gqa_step leaves them
 //   k_kv8_prefill  a prompt's portion
-// Scores are whole: a query is cut into balanced digits of 8 bits with one scale (23 bits in a step, 15 in a prompt, whose queries are bf16), the products with the keys'
-// numbers are exact in 32-bit integers, and the scales come behind them.  A weight times its value's scale meets the values' numbers as f16, which holds them exactly: a
-// (high, low) pair in a step, one f16 in a prompt (2^-12 against the 2^-9 of its bf16 output).
+// A step's scores are whole: a query is cut into three balanced digits of 8 bits with one scale (23 bits), the products with the keys' numbers are exact in 32-bit integers, and
+// the scales come behind them; a weight times its value's scale meets the values' numbers, which f16 holds exactly, as a (high, low) pair of f16.  A prompt's queries are bf16 and
+// so are its outputs: f16 throughout (see there).
 #include "gqa.hpp"
 
 namespace bitnet_hip {
@@ -36,16 +36,21 @@ __device__ __forceinline__ f16x8 eight_f16(uint32_t a, uint32_t b) {
     four_f16(b, x, y), v.z = x, v.w = y;
     return __builtin_bit_cast(f16x8, v);
 }
+// the same plus 1152: what a sum of them is too much by is taken off elsewhere
+__device__ __forceinline__ f16x8 eight_raised(uint32_t a, uint32_t b) {
+    const uint32_t u = a ^ 0x80808080u, v = b ^ 0x80808080u;
+    return __builtin_bit_cast(f16x8, u32x4{__builtin_amdgcn_perm(0x64646464u, u, 0x04010400u), __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u),
+                                           __builtin_amdgcn_perm(0x64646464u, v, 0x04010400u), __builtin_amdgcn_perm(0x64646464u, v, 0x04030402u)});
+}
+// the largest of three (an instruction by name: fmaxf would first make every operand canonical)
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
 // the least E with |v| < 2^E (v = 0: -100)
 __device__ __forceinline__ int exponent_above(float v) { return v > 0.f ? max(__builtin_amdgcn_frexp_expf(v), -100) : -100; }
 __device__ __forceinline__ float power2(int e) { return __builtin_amdgcn_ldexpf(1.0f, e); }
-
-// a product in which zero times anything is zero
-__device__ __forceinline__ float mul_zero(float a, float b) {
-    float r;
-    asm("v_mul_legacy_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
-    return r;
-}
 
 // where column c of a kv head's values at position pos lies
 __device__ __forceinline__ size_t kv8_value_at(int vdimp, int pos, int c) {
@@ -200,8 +205,7 @@ struct Kv8StepK {
     float *k_scale, *v_scale, *scratch, eps;
     int heads, group, dim, dimp, vdimp, capacity, turned, chunk, window, normed, append, k_at, v_at;  // normed: 1 queries, 2 keys
 };
-constexpr float kStepDigits = 8355000.0f;   // below 127 (2^16 + 2^8 + 1): three balanced digits
-constexpr float kPromptDigits = 32600.0f;   // below 127 (2^8 + 1): two
+constexpr float kStepDigits = 8355000.0f;  // below 127 (2^16 + 2^8 + 1): three balanced digits
 
 template <int NK, int NV, int MAPS>
 __global__ __launch_bounds__(256, NV > 8 || NK * MAPS >= 4 ? 1 : 2) void k_kv8_step(Kv8StepK p) {
@@ -527,294 +531,328 @@ hipError_t launch_kv8_step(const Kv8 &c, const GqaStep &a, hipStream_t s) {
 }
 
 // ---- prompt -----------------------------------------------------------------------------------------------------------
-// buffers of a tile in LDS: two where the tiles that are under way on a compute unit leave room
-constexpr int kv8_tile_bytes(int nk, int nv, int maps) { return maps * 64 * (nk * 64 + 32) + nv * 16 * (64 * 2 + 32) + (maps + 1) * 256 + 16; }
-constexpr int kv8_buffers(int nk, int nv, int maps) { return (nv > 8 || nk > 2 ? 2 : 4) * kv8_tile_bytes(nk, nv, maps) <= 163840 ? 2 : 1; }
+constexpr int kv8_tile_bytes(int nk, int nv, int maps) { return maps * 64 * (nk * 128 + 32) + nv * 16 * (64 * 2 + 32); }
+// A weight is exp2(score - m) times 2^kWeightUp, m being a maximum that follows the largest score once that is kLazy above it: at most 2^14.
+constexpr float kWeightUp = 6.0f, kLazy = 8.0f;
 
-// One workgroup: one head, four waves; a wave holds two slots of 16 queries: both maps of one query tile, or two tiles of the only map.  Key tiles of 64 (every map's) and the
-// values of the tile staged through registers into LDS one step ahead, the values as f16.  G = 2: two such groups of four waves share the keys of the same queries, tile by tile
-// in turn, and meet in LDS at the end.  records: gridDim.y workgroups share a block's tiles of keys, in stretches (launch_gqa_merge_parts).
-// A query of bf16 is two digits of 8 bits, 15 bits of its largest element.  l and o are held times 2^(14 - above), above being the exponent of the largest value scale so far.
+// One workgroup: the rows of W waves, a row being a query of one head; the heads that share keys and values are neighbours among the rows (row r: query r / group, head r % group of
+// the kv head).  A wave holds two slots of 16 rows: both maps of one set of rows, or two sets of the only map.  Key tiles of 64 (every map's) and the values of a tile are staged
+// through registers into LDS.  G = 2: two such groups of W waves share the keys of the same rows, tile by tile in turn, and meet in LDS at the end.  records: gridDim.y workgroups
+// share a block's tiles of keys, in stretches (launch_gqa_merge_parts).  MAPS = 1 with two maps, whose keys together find no room in LDS: gridDim.z is the map, with records.
+// In LDS keys are their numbers + 1152 as f16 (exact; a row's sum times 1152 is what its scores start from), and so is a query of bf16 times a power of two: scores are exact but
+// for the f32 sums, a key's scale meets them in f32.  Values are number times scale, brought under 2^15 by a power of two that holds for the group's tiles so far (`above`; o is
+// times 2^(8 - above)): a rounding of 2^-12 like that of the weights.  The sum of the weights is one more row of the products (ones times the same f16 weights).
+// The products of a SIMD's two waves and their vector instructions take about the same time, and as phases of their own they add up: hence the next tile's scores are made among
+// this tile's exponentials, and this tile's outputs among the staging of the tiles to come.
+// Wave 0 makes the values' factors two tiles ahead, wave 1 the keys' scales.  A value without a scale takes its key's away instead, so that only queries that see it lose theirs.
+// LDS of a tile: keys [maps][64][KS], values [columns][VS]; the 32 bytes behind a row of values hold the keys' scales (rows 16 s + 8 map .., s = 0
+// and 1 in turn), the factors (32 ..) and `above` (36).
 // FAR: with a distance penalty, gates per column, or both.
-template <int NK, int NV, int MAPS, bool FAR, int G>
-__global__ __launch_bounds__(256 * G, NV > 8 || NK > 2 ? 1 : 2) void k_kv8_prefill(Kv8 c, const uint16_t *Q, size_t ldq, int n_ctx, int nq, uint16_t *out, size_t ldo, int n_qb, float *records) {
+template <int NK, int NV, int MAPS, bool FAR, int G, int W>
+__global__ __launch_bounds__(64 * W * G, NV > 8 || NK > 2 ? 1 : 2) void k_kv8_prefill(Kv8 c, const uint16_t *Q, size_t ldq, int n_ctx, int nq, uint16_t *out, size_t ldo, int n_qb, float *records) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-    constexpr int SLOTS = 2, QW = 16 * SLOTS / MAPS, KS = NK * 64 + 32, VS = 64 * 2 + 32, NVL = NV / 4;
+    constexpr int SLOTS = 2, QW = 16 * SLOTS / MAPS, KK = 2 * NK, KS = NK * 128 + 32, VS = 64 * 2 + 32, T = 64 * W, KC = NK * 4, KR = T / KC, NKL = (MAPS * 64 + KR - 1) / KR, NVL = (NV * 64 + T - 1) / T;
+    constexpr int KB = MAPS * 64 * KS, TILE = kv8_tile_bytes(NK, NV, MAPS), PAD = KB + 128;
     const Gqa &p = c.g;
-    const int grp = G == 2 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 8) : 0, tid = threadIdx.x & 255, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r16 = lane & 15, g = lane >> 4;
-    constexpr int KB = MAPS * 64 * KS, SB = KB + NV * 16 * VS, TILE = kv8_tile_bytes(NK, NV, MAPS), BUFS = kv8_buffers(NK, NV, MAPS);
-    uint8_t *lk = lds + grp * BUFS * TILE;
-    const int heads = (int)p.heads, dimp = (int)p.dimp, vdimp = (int)p.vdimp;
-    // (the order of k_gqa_prefill's workgroups)
-    const int x = blockIdx.x & 7, rest = blockIdx.x >> 3, own = heads >> 3, left = heads & 7, per = own + (left ? 1 : 0);
-    const int level = rest / per, slot = rest - level * per, r = (x + 8 * left - (level % 8) * left) & 7;
-    if (slot == own && r >= left) return;
-    const int h = slot < own ? x * own + slot : 8 * own + r, qb = n_qb - 1 - level;
-    const int kv = h / (int)(p.heads / p.kv_heads), q0 = qb * 4 * QW, pos0 = n_ctx - nq, qw = q0 + wave * QW;
-    i32x4 qd[SLOTS][2][NK];  // digits: low, high
-    float qs[SLOTS];
-    int qpos[SLOTS], qfirst[SLOTS];
+    const int grp = G == 2 ? __builtin_amdgcn_readfirstlane(threadIdx.x / T) : 0, tid = threadIdx.x & (T - 1), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r16 = lane & 15, g = lane >> 4;
+    uint8_t *lk = lds + grp * 2 * TILE;
+    const int heads = (int)p.heads, kv_heads = (int)p.kv_heads, group = heads / kv_heads, dimp = (int)p.dimp, vdimp = (int)p.vdimp;
+    // longest blocks first; consecutive workgroups go to the eight XCDs in turn
+    const int level = blockIdx.x / kv_heads, kv = blockIdx.x - level * kv_heads, qb = n_qb - 1 - level, maps = MAPS == 1 ? (int)p.maps : MAPS, alone = MAPS == 1 ? (int)blockIdx.z : 0;
+    const int pos0 = n_ctx - nq, row0 = qb * W * QW, rw = row0 + wave * QW, last = nq - 1;
+    const int q_lo = min(rw / group, last), q_hi = min((rw + QW - 1) / group, last), q_first = row0 / group, q_last = min((row0 + W * QW - 1) / group, last);
+    f16x8 qf[SLOTS][KK];
+    float qs[SLOTS], raised[SLOTS], m[SLOTS];
+    FarPenalty far[SLOTS / MAPS];
+    int qpos[SLOTS], qfirst[SLOTS], head[SLOTS / MAPS];
+    f32x4 o[NV][SLOTS], l[SLOTS];
 #pragma unroll
     for (int t = 0; t < SLOTS; ++t) {
-        const int tile = t / MAPS, map = t % MAPS, qi = min(qw + tile * 16 + r16, nq - 1);
-        qpos[t] = pos0 + qw + tile * 16 + r16;
-        qfirst[t] = gqa_first(p, qpos[t]);
-        const uint16_t *q = Q + (size_t)qi * ldq + (size_t)(h * MAPS + map) * dimp;
-        float largest = 0.f;
-        u32x4 raw[NK][2];
+        const int at = rw + t / MAPS * 16 + r16, qi = min(at / group, last), h = kv * group + at % group, map = alone + t % MAPS;
+        head[t / MAPS] = h, qpos[t] = pos0 + qi, qfirst[t] = gqa_first(p, qpos[t]);
+        const uint16_t *q = Q + (size_t)qi * ldq + (size_t)(h * maps + map) * dimp;
+        float largest = 0.f, total = 0.f, v[KK][8];
 #pragma unroll
-        for (int kk = 0; kk < NK; ++kk)
+        for (int kk = 0; kk < KK; ++kk) {
+            const u32x4 raw = kk * 32 < dimp ? *reinterpret_cast<const u32x4 *>(q + kk * 32 + g * 8) : u32x4{0u, 0u, 0u, 0u};
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                raw[kk][e] = kk * 64 + g * 16 < dimp ? *reinterpret_cast<const u32x4 *>(q + kk * 64 + g * 16 + e * 8) : u32x4{0u, 0u, 0u, 0u};
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float v = bf2f(raw[kk][e][i >> 1] >> (16 * (i & 1)) & 0xffffu);
-                    largest = fmaxf(largest, is_finite(v) ? fabsf(v) : INFINITY);
-                }
+            for (int i = 0; i < 8; ++i) {
+                v[kk][i] = bf2f(raw[i >> 1] >> (16 * (i & 1)) & 0xffffu);
+                largest = fmaxf(largest, is_finite(v[kk][i]) ? fabsf(v[kk][i]) : INFINITY);
             }
+        }
         largest = rows_max(largest);
-        const bool live = largest >= 1e-30f && is_finite(largest);
-        const float to = live ? kPromptDigits / largest : 0.f;
-        qs[t] = live ? largest * (kLog2e / kPromptDigits) : is_finite(largest) ? 1.0f : __builtin_nanf("");
+        const int e = min(max(exponent_above(largest), -50), 100);
+        qs[t] = is_finite(largest) ? kLog2e * power2(e - 12) : __builtin_nanf("");
 #pragma unroll
-        for (int kk = 0; kk < NK; ++kk)
+        for (int kk = 0; kk < KK; ++kk)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                uint32_t lo = 0, hi = 0;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int at = 4 * i + e;
-                    const float v = bf2f(raw[kk][at >> 3][(at & 7) >> 1] >> (16 * (at & 1)) & 0xffffu);
-                    const int n = live ? (int)rintf(v * to) : 0, d0 = (int)(int8_t)n, d1 = (n - d0) >> 8;
-                    lo |= (uint32_t)(d0 & 0xff) << (8 * e), hi |= (uint32_t)(d1 & 0xff) << (8 * e);
-                }
-                qd[t][0][kk][i] = (int)lo, qd[t][1][kk][i] = (int)hi;
+            for (int i = 0; i < 8; ++i) {
+                qf[t][kk][i] = (_Float16)(is_finite(largest) ? __builtin_amdgcn_ldexpf(v[kk][i], 12 - e) : 0.f);
+                total += (float)qf[t][kk][i];
             }
-    }
-    f32x4 o[NV][SLOTS];
-    float m[SLOTS], l[SLOTS];
-    int above = -80;
-#pragma unroll
-    for (int t = 0; t < SLOTS; ++t) {
-        // (finite: with chunks a tile may hold no key that a query sees; the sink counts once per query, four lanes share one)
+        raised[t] = -1152.0f * rows_sum(total);
+        // (finite: with chunks a tile may hold no key that a query sees)
         const bool sink = MAPS == 1 && p.sink && grp == 0 && !records;
-        m[t] = sink ? p.sink[h] * kLog2e : -1e30f, l[t] = sink && g == 0 ? power2(14 - above) : 0.f;
+        m[t] = sink ? p.sink[h] * kLog2e : -1e30f;
+        if (FAR && MAPS == 1) far[t] = far_penalty(p, h), far[t].weight *= kLog2e;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) l[t][i] = sink ? power2((int)kWeightUp) : 0.f;
 #pragma unroll
         for (int v = 0; v < NV; ++v) o[v][t] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    const int8_t *K = (const int8_t *)p.kcache + (size_t)kv * MAPS * p.capacity * dimp, *V = (const int8_t *)p.vcache + (size_t)kv * vdimp * p.capacity;
-    const float *KSC = c.k_scale + (size_t)kv * MAPS * p.capacity, *VSC = c.v_scale + (size_t)kv * p.capacity;
+    int above = -60;
+    const int8_t *K = (const int8_t *)p.kcache + (size_t)(kv * maps + alone) * p.capacity * dimp, *V = (const int8_t *)p.vcache + (size_t)kv * vdimp * p.capacity;
+    const float *KSC = c.k_scale + (size_t)(kv * maps + alone) * p.capacity, *VSC = c.v_scale + (size_t)kv * p.capacity;
     // keys: a row of the tile by KC neighbouring threads; row p of 32 in LDS is key 8 (p >> 2 & 3) + 4 (p >> 4) + (p & 3)
-    constexpr int KC = NK * 4, KR = 256 / KC;
-    u32x4 kreg[MAPS][NK], vreg[NVL];
-    float sreg[MAPS + 1];
-    const unsigned koff = (unsigned)((tid / KC) * dimp + min((tid % KC) * 16, dimp - 16));
-    int kw[NK], vw[NVL], voff[NVL];
+    u32x4 kreg[NKL], vreg[NVL];
+    float kscale[MAPS], vscale = 0.f, vnan = 0.f;
+    int kw[NKL], vw[NVL], voff[NVL], vf[NVL];
+    unsigned koff[NKL];
 #pragma unroll
-    for (int j = 0; j < NK; ++j) {
-        const int key = tid / KC + j * KR, row = (key & 32) + (key >> 2 & 1) * 16 + (key >> 3 & 3) * 4 + (key & 3);
-        kw[j] = row * KS + (tid % KC) * 16;
+    for (int j = 0; j < NKL; ++j) {
+        const int at = min(tid / KC + j * KR, MAPS * 64 - 1), key = at & 63, mp = at >> 6, row = (key & 32) + (key >> 2 & 1) * 16 + (key >> 3 & 3) * 4 + (key & 3);
+        kw[j] = (mp * 64 + row) * KS + (tid % KC) * 32;
+        koff[j] = (unsigned)(key * dimp + min((tid % KC) * 16, dimp - 16));
     }
 #pragma unroll
     for (int j = 0; j < NVL; ++j) {  // sixteen bytes: eight keys of two columns, 16 apart; columns past vdimp are zero
-        const int i = tid + 256 * j, half = i / (NV * 32), rem = i % (NV * 32);
-        vw[j] = KB + ((rem >> 6) * 32 + (rem >> 2 & 15)) * VS + half * 64 + (rem & 3) * 16;
+        const int i = tid + T * j, half = i / (NV * 32) & 1, rem = i % (NV * 32), key = half * 32 + (rem & 3) * 8;
+        vw[j] = KB + ((rem >> 6) * 32 + (rem >> 2 & 15)) * VS + key * 2;
         voff[j] = (rem >> 6) * 32 < vdimp ? half * vdimp * 32 + rem * 16 : -1;
+        vf[j] = PAD + (32 + (key >> 4)) * VS + (key & 8) * 2;
         vreg[j] = u32x4{0u, 0u, 0u, 0u};
     }
-    auto fetch = [&](int key0) {  // (whole tiles: the capacity is a multiple of 64)
-#pragma unroll
-        for (int mp = 0; mp < MAPS; ++mp) {
-            const int8_t *kb = K + ((size_t)mp * p.capacity + key0) * dimp;
-#pragma unroll
-            for (int j = 0; j < NK; ++j) kreg[mp][j] = *reinterpret_cast<const u32x4 *>(kb + (size_t)(j * KR) * dimp + koff);
-        }
-        const int8_t *vb = V + (size_t)key0 * vdimp;
-#pragma unroll
-        for (int j = 0; j < NVL; ++j)
-            if (voff[j] >= 0) vreg[j] = *reinterpret_cast<const u32x4 *>(vb + voff[j]);
-        if (wave == 0) {  // (a position past the portion may hold anything)
-            const bool in = key0 + lane < n_ctx;
-#pragma unroll
-            for (int mp = 0; mp < MAPS; ++mp) sreg[mp] = in ? KSC[(size_t)mp * p.capacity + key0 + lane] : 0.f;
-            sreg[MAPS] = in ? VSC[key0 + lane] : 0.f;
-        }
-    };
-    auto store = [&](int at) {
-#pragma unroll
-        for (int mp = 0; mp < MAPS; ++mp)
-#pragma unroll
-            for (int j = 0; j < NK; ++j) *reinterpret_cast<u32x4 *>(lk + at + kw[j] + mp * 64 * KS) = kreg[mp][j];
-#pragma unroll
-        for (int j = 0; j < NVL; ++j) {
-            *reinterpret_cast<f16x8 *>(lk + at + vw[j]) = eight_f16(vreg[j].x, vreg[j].y);
-            *reinterpret_cast<f16x8 *>(lk + at + vw[j] + 16 * VS) = eight_f16(vreg[j].z, vreg[j].w);
-        }
-        if (wave == 0) {
-            float *sc = reinterpret_cast<float *>(lk + at + SB);
-#pragma unroll
-            for (int mp = 0; mp <= MAPS; ++mp) sc[mp * 64 + lane] = sreg[mp];
-            const int e = min(exponent_above(rows_max(row_max(fmaxf(sreg[MAPS], 0.f)))), 126);
-            if (lane == 0) reinterpret_cast<int *>(sc)[(MAPS + 1) * 64] = e;
-        }
-    };
-    int n_tiles = (min(n_ctx, pos0 + q0 + 4 * QW) + 63) / 64;
-    const FarPenalty far = far_penalty(p, h);
-    // tiles from the first key of the workgroup's first query on; a wave leaves out what lies ahead of its own first key
-    int t_first = gqa_first(p, pos0 + q0) >> 6;
-    const int w_first = gqa_first(p, pos0 + qw), w_last = gqa_first(p, pos0 + qw + QW - 1);
+    int t_first = gqa_first(p, pos0 + q_first) >> 6, n_tiles = (pos0 + q_last) / 64 + 1;
+    const int w_last = gqa_first(p, pos0 + q_hi);
     if (records) {
         const int each = (n_tiles - t_first + (int)gridDim.y - 1) / (int)gridDim.y;
         t_first = min(t_first + (int)blockIdx.y * each, n_tiles), n_tiles = min(t_first + each, n_tiles);
     }
-    fetch(max(min(t_first + grp, n_tiles - 1), 0) * 64);
-    if (BUFS == 2) {
-        store(0);
-        if (t_first + grp + G < n_tiles) fetch((t_first + grp + G) * 64);
-    }
-    int at = 0;  // the tile's buffer
-    for (int t0 = t_first; t0 < n_tiles; t0 += G) {
-        const int kt0 = t0 + grp, key0 = kt0 * 64;
-        __syncthreads();
-        if (BUFS == 1) {
-            store(0);
-            __syncthreads();
-            if (kt0 + G < n_tiles) fetch(key0 + G * 64);
+    const int end = n_tiles * 64 - 1;
+    // The group's i-th tile; what lies past the last one is read from the last one, and all of it hidden.
+    auto first_key = [&](int i) { return max(min(t_first + grp + G * i, n_tiles - 1), 0) * 64; };
+    constexpr bool whole_keys = NKL * KR == MAPS * 64, whole_values = NVL * T == NV * 64;
+    auto fetch_keys = [&](int i) {  // (whole tiles: the capacity is a multiple of 64)
+        const int key0 = first_key(i);
+#pragma unroll
+        for (int j = 0; j < NKL; ++j) {
+            const int mp = MAPS == 1 ? 0 : (tid / KC + j * KR) >> 6 & 1;
+            if (whole_keys || tid / KC + j * KR < MAPS * 64) kreg[j] = *reinterpret_cast<const u32x4 *>(K + ((size_t)mp * p.capacity + key0) * dimp + koff[j]);
         }
-        const bool seen = !(key0 > pos0 + qw + QW - 1 || key0 + 63 < w_first || (G == 2 && kt0 >= n_tiles));  // (else: no key of the tile is seen by this wave's queries)
-        const uint8_t *kt_ = lk + at;
-        f16x8 pf[2][SLOTS];
-        if (seen) {
-            const float *sc = reinterpret_cast<const float *>(kt_ + SB);
-            const int need = __builtin_amdgcn_readfirstlane(reinterpret_cast<const int *>(sc)[(MAPS + 1) * 64]);
-            if (need > above) {
-                const float down = power2(above - need);
+        if (wave == 1) {
+            const bool in = key0 + lane < n_ctx;  // (a position past the portion may hold anything)
 #pragma unroll
-                for (int t = 0; t < SLOTS; ++t) {
-                    l[t] *= down;
-#pragma unroll
-                    for (int v = 0; v < NV; ++v) o[v][t] *= down;
-                }
-                above = need;
-            }
-            f32x4 s[4][SLOTS];
-#pragma unroll
-            for (int kt = 0; kt < 4; ++kt) {
-                i32x4 a[SLOTS][2];
-#pragma unroll
-                for (int t = 0; t < SLOTS; ++t) a[t][0] = a[t][1] = i32x4{0, 0, 0, 0};
-#pragma unroll
-                for (int kk = 0; kk < NK; ++kk)
-#pragma unroll
-                    for (int t = 0; t < SLOTS; ++t) {
-                        const i32x4 k = *reinterpret_cast<const i32x4 *>(kt_ + ((t % MAPS) * 64 + kt * 16 + r16) * KS + kk * 64 + g * 16);
-                        a[t][0] = mfma_i8(k, qd[t][0][kk], a[t][0]);
-                        a[t][1] = mfma_i8(k, qd[t][1][kk], a[t][1]);
-                    }
-#pragma unroll
-                for (int t = 0; t < SLOTS; ++t) {
-                    const f32x4 ks = *reinterpret_cast<const f32x4 *>(sc + (t % MAPS) * 64 + (kt >> 1) * 32 + g * 8 + (kt & 1) * 4);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) s[kt][t][i] = (float)(a[t][1][i] * 256 + a[t][0][i]) * ks[i];
-                }
-            }
-            // (from here on a score is times qs, which holds log2(e))
-            if (FAR && p.far_weight)
-#pragma unroll
-                for (int t = 0; t < SLOTS; ++t)
-#pragma unroll
-                    for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            s[kt][t][i] = nearer(s[kt][t][i] * qs[t], FarPenalty{far.weight * kLog2e, far.rate}, qpos[t] - (key0 + (kt >> 1) * 32 + g * 8 + (kt & 1) * 4 + i));
-            if (key0 + 63 > pos0 + qw)  // the diagonal
-#pragma unroll
-                for (int t = 0; t < SLOTS; ++t)
-#pragma unroll
-                    for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) s[kt][t][i] = key0 + (kt >> 1) * 32 + g * 8 + (kt & 1) * 4 + i > qpos[t] ? -INFINITY : s[kt][t][i];
-            if (key0 < w_last)  // an earlier chunk of some of the queries
-#pragma unroll
-                for (int t = 0; t < SLOTS; ++t)
-#pragma unroll
-                    for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) s[kt][t][i] = key0 + (kt >> 1) * 32 + g * 8 + (kt & 1) * 4 + i < qfirst[t] ? -INFINITY : s[kt][t][i];
-            float mn[SLOTS], c2[SLOTS];
-            bool grows = false;
-#pragma unroll
-            for (int t = 0; t < SLOTS; ++t) {
-                c2[t] = FAR && p.far_weight ? 1.0f : qs[t];
-                float mx = fmaxf(fmaxf(s[0][t][0], s[0][t][1]), fmaxf(s[0][t][2], s[0][t][3]));
-#pragma unroll
-                for (int kt = 1; kt < 4; ++kt) mx = fmaxf(mx, fmaxf(fmaxf(s[kt][t][0], s[kt][t][1]), fmaxf(s[kt][t][2], s[kt][t][3])));
-                mn[t] = fmaxf(m[t], rows_max(mx) * c2[t]);
-                grows = grows || mn[t] > m[t];
-            }
-            if (__any(grows)) {
-#pragma unroll
-                for (int t = 0; t < SLOTS; ++t) {
-                    const float al = __builtin_amdgcn_exp2f(m[t] - mn[t]);
-                    m[t] = mn[t];
-                    l[t] *= al;
-#pragma unroll
-                    for (int v = 0; v < NV; ++v) o[v][t] *= al;
-                }
-            }
-#pragma unroll
-            for (int ks = 0; ks < 2; ++ks) {
-                f32x4 vs[2];
-#pragma unroll
-                for (int j = 0; j < 2; ++j) vs[j] = *reinterpret_cast<const f32x4 *>(sc + MAPS * 64 + ks * 32 + g * 8 + j * 4);
-#pragma unroll
-                for (int t = 0; t < SLOTS; ++t)
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        f32x4 w;
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) w[i] = __builtin_amdgcn_exp2f(fmaf(s[2 * ks + j][t][i], c2[t], (float)(14 - above) - m[t]));
-                        l[t] += (w[0] + w[1]) + (w[2] + w[3]);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) pf[ks][t][4 * j + i] = (_Float16)mul_zero(w[i], vs[j][i]);  // (a value that the mask hides may have no number for a scale)
-                    }
-            }
+            for (int mp = 0; mp < MAPS; ++mp) kscale[mp] = in ? KSC[(size_t)mp * p.capacity + key0 + lane] : 0.f;
+            vnan = in ? VSC[key0 + lane] : 0.f;
         }
-        if (BUFS == 2) {
-            at ^= TILE;
-            if (kt0 + G < n_tiles) store(at);
-            if (kt0 + 2 * G < n_tiles) fetch(key0 + 2 * G * 64);
+    };
+    auto fetch_values = [&](int i) {
+        const int8_t *vb = V + (size_t)first_key(i) * vdimp;
+#pragma unroll
+        for (int j = 0; j < NVL; ++j)
+            if (voff[j] >= 0 && (whole_values || tid + T * j < NV * 64)) vreg[j] = *reinterpret_cast<const u32x4 *>(vb + voff[j]);
+    };
+    auto fetch_factors = [&](int i) {
+        if (wave == 0) {
+            const int key0 = first_key(i);
+            vscale = key0 + lane < n_ctx ? VSC[key0 + lane] : 0.f;
         }
-        if (seen)
+    };
+    int highest = -60;
+    auto publish = [&](int i) {  // the factors of tile i
+        if (wave == 0) {
+            const float v = fmaxf(vscale, 0.f);
+            highest = max(highest, __builtin_amdgcn_readfirstlane(min(exponent_above(rows_max(row_max(v))), 126)));
+            uint8_t *dst = lk + (i & 1) * TILE + PAD;
+            *reinterpret_cast<_Float16 *>(dst + (32 + (lane >> 4)) * VS + (lane & 15) * 2) = (_Float16)__builtin_amdgcn_ldexpf(v, 8 - highest);
+            if (lane == 0) *reinterpret_cast<int *>(dst + 36 * VS + (i >> 1 & 1) * 4) = highest;
+        }
+    };
+    // stores go by pieces of eight numbers a thread, 2 NKL and 2 NVL of them
+    auto store_keys = [&](int i, int u) {
+        uint8_t *dst = lk + (i & 1) * TILE;
+        const int j = u >> 1;
+        if (whole_keys || tid / KC + j * KR < MAPS * 64) *reinterpret_cast<f16x8 *>(dst + kw[j] + (u & 1) * 16) = u & 1 ? eight_raised(kreg[j].z, kreg[j].w) : eight_raised(kreg[j].x, kreg[j].y);
+        if (u == 2 * NKL - 1 && wave == 1)
 #pragma unroll
-            for (int v = 0; v < NV; ++v)
+            for (int mp = 0; mp < MAPS; ++mp)
+                *reinterpret_cast<float *>(dst + PAD + ((i >> 1 & 1) * 16 + 8 * mp + (lane >> 3)) * VS + (lane & 7) * 4) = vnan == vnan ? kscale[mp] : vnan;
+    };
+    f16x8 factor[NVL];
+    auto read_factors = [&](int i) {
 #pragma unroll
-                for (int ks = 0; ks < 2; ++ks) {
-                    const f16x8 a = *reinterpret_cast<const f16x8 *>(kt_ + KB + (v * 16 + r16) * VS + ks * 64 + g * 16);
+        for (int j = 0; j < NVL; ++j)
+            if (whole_values || tid + T * j < NV * 64) factor[j] = *reinterpret_cast<const f16x8 *>(lk + (i & 1) * TILE + vf[j]);
+    };
+    auto store_values = [&](int i, int u) {
+        const int j = u >> 1;
+        if (whole_values || tid + T * j < NV * 64)
+            *reinterpret_cast<f16x8 *>(lk + (i & 1) * TILE + vw[j] + (u & 1) * 16 * VS) = (u & 1 ? eight_f16(vreg[j].z, vreg[j].w) : eight_f16(vreg[j].x, vreg[j].y)) * factor[j];
+    };
+    const int steps = (n_tiles - t_first + G - 1) / G;
+    // keys of tiles 0 and 1, values of tile 0, factors of tiles 0 and 1
+    fetch_keys(0), fetch_values(0), fetch_factors(0);
+    publish(0);
+    fetch_factors(1);
 #pragma unroll
-                    for (int t = 0; t < SLOTS; ++t) o[v][t] = mfma_f16(a, pf[ks][t], o[v][t]);
-                }
-    }
-    {
-        const float back = power2(above - 14);
+    for (int u = 0; u < 2 * NKL; ++u) store_keys(0, u);
+    fetch_keys(1);
+    __syncthreads();
+    publish(1);
+    fetch_factors(2);
+    read_factors(0);
+#pragma unroll
+    for (int u = 0; u < 2 * NVL; ++u) store_values(0, u);
+    fetch_values(1);
+#pragma unroll
+    for (int u = 0; u < 2 * NKL; ++u) store_keys(1, u);
+    fetch_keys(2);
+    // Scores go by halves of a tile (32 keys): of the half at hand and of the next one, times their keys' scales, in units of qs, which holds log2(e).
+    f32x4 s0[2][SLOTS], s1[2][SLOTS];
+    float mx[SLOTS];  // the largest of the lane's
+    constexpr int KREADS = 2 * KK * MAPS, AHEAD = 4;
+    // operand j of a half's scores, and what it is multiplied with
+    auto key_operand = [&](const uint8_t *tile, int half, int j) {
+        const int kk = j / (2 * MAPS), kt = j / MAPS % 2, mp = j % MAPS;
+        return *reinterpret_cast<const f16x8 *>(tile + (mp * 64 + half * 32 + kt * 16 + r16) * KS + kk * 64 + g * 16);
+    };
+    auto key_products = [&](const f16x8 &k, int j, f32x4 (&to)[2][SLOTS]) {
+        const int kk = j / (2 * MAPS), kt = j / MAPS % 2, mp = j % MAPS;
 #pragma unroll
         for (int t = 0; t < SLOTS; ++t) {
-            l[t] *= back;
-#pragma unroll
-            for (int v = 0; v < NV; ++v) o[v][t] *= back;
+            if (MAPS == 2 && t != mp) continue;
+            if (kk == 0) to[kt][t] = f32x4{raised[t], raised[t], raised[t], raised[t]};
+            to[kt][t] = mfma_f16(k, qf[t][kk], to[kt][t]);
         }
+    };
+    auto value_operand = [&](const uint8_t *tile, int half, int j) { return *reinterpret_cast<const f16x8 *>(tile + KB + (j * 16 + r16) * VS + half * 64 + g * 16); };
+    // the j-th quarter of a half's scores: their keys' scales and the largest
+    auto scaled = [&](const uint8_t *tile, int i, int half, int j, f32x4 (&of)[2][SLOTS]) {
+        const int kt = j / SLOTS, t = j % SLOTS;
+        of[kt][t] *= *reinterpret_cast<const f32x4 *>(tile + PAD + ((i >> 1 & 1) * 16 + 8 * (t % MAPS) + half * 4 + g) * VS + kt * 16);
+        mx[t] = kt == 0 ? max3(of[kt][t][0], of[kt][t][1], of[kt][t][2]) : max3(mx[t], of[kt][t][0], of[kt][t][1]);
+        mx[t] = kt == 0 ? max3(mx[t], of[kt][t][3], of[kt][t][3]) : max3(mx[t], of[kt][t][2], of[kt][t][3]);
+    };
+#pragma unroll
+    for (int j = 0; j < KREADS; ++j) key_products(key_operand(lk, 0, j), j, s0);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) scaled(lk, 0, 0, j, s0);
+    f16x8 one;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) one[i] = (_Float16)1.0f;
+    // half `half` of tile i, its scores in s; the half behind it, of tile ni, into ahead
+    auto step = [&](int i, int half, int need, f32x4 (&s)[2][SLOTS], f32x4 (&ahead)[2][SLOTS]) __attribute__((always_inline)) {
+        const int key0 = (t_first + grp + G * i) * 64 + half * 32, ni = i + half, other = half ^ 1;
+        const uint8_t *here = lk + (i & 1) * TILE, *next = lk + (ni & 1) * TILE;
+        if (key0 + 31 > min(pos0 + q_lo, end) || key0 < w_last || (FAR && p.far_weight))  // (the diagonal or what lies past the last tile; an earlier chunk of some of the queries)
+#pragma unroll
+            for (int t = 0; t < SLOTS; ++t) {
+                mx[t] = -INFINITY;
+#pragma unroll
+                for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int key = key0 + g * 8 + kt * 4 + e;
+                        float v = s[kt][t][e];
+                        if (FAR && p.far_weight) v = nearer(v * qs[t], far[t / MAPS], max(qpos[t] - key, 0));
+                        s[kt][t][e] = v = key > min(qpos[t], end) || key < qfirst[t] ? -INFINITY : v;
+                        mx[t] = fmaxf(mx[t], v);
+                    }
+            }
+        float c2[SLOTS];
+        bool grows = need > above;
+#pragma unroll
+        for (int t = 0; t < SLOTS; ++t) {
+            c2[t] = FAR && p.far_weight ? 1.0f : qs[t];
+            grows = grows || mx[t] * c2[t] > m[t] + kLazy;
+        }
+        if (__any(grows)) {
+            const float down = power2(min(above - need, 0));
+            above = max(above, need);
+#pragma unroll
+            for (int t = 0; t < SLOTS; ++t) {
+                const float largest = rows_max(mx[t]) * c2[t], to = largest > m[t] + kLazy ? largest : m[t], al = __builtin_amdgcn_exp2f(m[t] - to);
+                m[t] = to;
+                l[t] *= al;
+#pragma unroll
+                for (int v = 0; v < NV; ++v) o[v][t] *= al * down;
+            }
+        }
+        if (half == 0) read_factors(i + 1);
+        u32x4 w[SLOTS];
+        {
+            f16x8 k[KREADS];
+#pragma unroll
+            for (int j = 0; j < AHEAD; ++j) k[j] = key_operand(next, other, j);
+#pragma unroll
+            for (int j = 0; j < KREADS; ++j) {
+                __builtin_amdgcn_sched_barrier(0);
+                if (j + AHEAD < KREADS) k[j + AHEAD] = key_operand(next, other, j + AHEAD);
+                key_products(k[j], j, ahead);
+#pragma unroll
+                for (int u = j * 8 / KREADS; u < (j + 1) * 8 / KREADS; ++u) {  // two weights
+                    const int t = u >> 2, e = u & 3;
+                    const float off = kWeightUp - m[t];
+                    const float a = __builtin_amdgcn_exp2f(fmaf(s[e >> 1][t][2 * e & 3], c2[t], off)), b = __builtin_amdgcn_exp2f(fmaf(s[e >> 1][t][(2 * e & 3) + 1], c2[t], off));
+                    w[t][e] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));  // (cut off, in the sum as in the products)
+                }
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        {
+            f16x8 v[NV];
+#pragma unroll
+            for (int j = 0; j < AHEAD; ++j) v[j] = value_operand(here, half, j);
+#pragma unroll
+            for (int t = 0; t < SLOTS; ++t) l[t] = mfma_f16(one, __builtin_bit_cast(f16x8, w[t]), l[t]);
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                __builtin_amdgcn_sched_barrier(0);
+                if (j + AHEAD < NV) v[j + AHEAD] = value_operand(here, half, j + AHEAD);
+#pragma unroll
+                for (int t = 0; t < SLOTS; ++t) o[j][t] = mfma_f16(v[j], __builtin_bit_cast(f16x8, w[t]), o[j][t]);
+#pragma unroll
+                for (int u = j * 4 / NV; u < (j + 1) * 4 / NV; ++u) scaled(next, ni, other, u, ahead);
+                constexpr int VP = 2 * NVL, KP = 2 * NKL;
+#pragma unroll
+                for (int u = j * VP / NV; half == 0 && u < (j + 1) * VP / NV; ++u) store_values(i + 1, u);
+#pragma unroll
+                for (int u = j * KP / NV; half == 1 && u < (j + 1) * KP / NV; ++u) store_keys(i + 2, u);
+            }
+            if (half == 0)
+                fetch_values(i + 2);
+            else
+                fetch_keys(i + 3);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    for (int i = 0; i < steps; ++i) {
+        __syncthreads();
+        publish(i + 2);
+        fetch_factors(i + 3);
+        const int need = __builtin_amdgcn_readfirstlane(*reinterpret_cast<const int *>(lk + (i & 1) * TILE + PAD + 36 * VS + (i >> 1 & 1) * 4));
+        step(i, 0, need, s0, s1);
+        step(i, 1, need, s1, s0);
+    }
+    float sum[SLOTS];
+#pragma unroll
+    for (int t = 0; t < SLOTS; ++t) {
+        const float back = power2(above - 8 - (int)kWeightUp);
+        sum[t] = l[t].x * power2(-(int)kWeightUp);
+#pragma unroll
+        for (int v = 0; v < NV; ++v) o[v][t] *= back;
     }
     if (G == 2) {
         f32x4 *po = reinterpret_cast<f32x4 *>(lds);                                       // [wave][slot][NV][lane]
-        float2 *pm = reinterpret_cast<float2 *>(lds + (size_t)4 * SLOTS * NV * 64 * 16);  // [wave][slot][lane]
+        float2 *pm = reinterpret_cast<float2 *>(lds + (size_t)W * SLOTS * NV * 64 * 16);  // [wave][slot][lane]
         __syncthreads();
         if (grp == 1) {
 #pragma unroll
             for (int t = 0; t < SLOTS; ++t) {
 #pragma unroll
                 for (int v = 0; v < NV; ++v) po[((wave * SLOTS + t) * NV + v) * 64 + lane] = o[v][t];
-                pm[(wave * SLOTS + t) * 64 + lane] = float2{m[t], l[t]};
+                pm[(wave * SLOTS + t) * 64 + lane] = float2{m[t], sum[t]};
             }
         }
         __syncthreads();
@@ -823,7 +861,7 @@ __global__ __launch_bounds__(256 * G, NV > 8 || NK > 2 ? 1 : 2) void k_kv8_prefi
         for (int t = 0; t < SLOTS; ++t) {
             const float2 b = pm[(wave * SLOTS + t) * 64 + lane];
             const float mx = fmaxf(m[t], b.x), wa = __builtin_amdgcn_exp2f(m[t] - mx), wb = __builtin_amdgcn_exp2f(b.x - mx);
-            m[t] = mx, l[t] = l[t] * wa + b.y * wb;
+            m[t] = mx, sum[t] = sum[t] * wa + b.y * wb;
 #pragma unroll
             for (int v = 0; v < NV; ++v) o[v][t] = o[v][t] * wa + po[((wave * SLOTS + t) * NV + v) * 64 + lane] * wb;
         }
@@ -831,25 +869,19 @@ __global__ __launch_bounds__(256 * G, NV > 8 || NK > 2 ? 1 : 2) void k_kv8_prefi
     if (records) {
 #pragma unroll
         for (int t = 0; t < SLOTS; ++t) {
-            const int qi = qw + t / MAPS * 16 + r16;
-            const float sum = rows_sum(l[t]);
-            if (qi >= nq) continue;
-            float *rec = records + ((((size_t)qi * heads + h) * MAPS + t % MAPS) * gridDim.y + blockIdx.y) * (kGqaRecHead + vdimp);
-            if (g == 0) rec[0] = m[t], rec[1] = sum;
+            const int at = rw + t / MAPS * 16 + r16;
+            if (at >= nq * group) continue;
+            float *rec = records + ((((size_t)(at / group) * heads + head[t / MAPS]) * maps + alone + t % MAPS) * gridDim.y + blockIdx.y) * (kGqaRecHead + vdimp);
+            if (g == 0) rec[0] = m[t], rec[1] = sum[t];
 #pragma unroll
             for (int v = 0; v < NV; ++v)
                 if (v * 16 < vdimp) *reinterpret_cast<f32x4 *>(rec + kGqaRecHead + v * 16 + g * 4) = o[v][t];
         }
         return;
     }
-    float inv[SLOTS], gate[SLOTS / MAPS];
+    float inv[SLOTS];
 #pragma unroll
-    for (int t = 0; t < SLOTS / MAPS; ++t) gate[t] = 1.0f;
-#pragma unroll
-    for (int t = 0; t < SLOTS; ++t) inv[t] = 1.0f / rows_sum(l[t]);
-    if (p.gate && !(FAR && p.gate_columns))
-#pragma unroll
-        for (int t = 0; t < SLOTS / MAPS; ++t) gate[t] = activate(gate_logit(p, min(qw + t * 16 + r16, nq - 1), h, 0), BITNET_HIP_ACT_SIGMOID);
+    for (int t = 0; t < SLOTS; ++t) inv[t] = 1.0f / sum[t];
     if (MAPS == 2) {
         float ss = 0.f;
 #pragma unroll
@@ -861,13 +893,14 @@ __global__ __launch_bounds__(256 * G, NV > 8 || NK > 2 ? 1 : 2) void k_kv8_prefi
     }
 #pragma unroll
     for (int t = 0; t < SLOTS / MAPS; ++t) {
-        const int qi = qw + t * 16 + r16;
-        if (qi >= nq) continue;
+        const int at = rw + t * 16 + r16, qi = at / group, h = head[t];
+        if (at >= nq * group) continue;
+        if (p.gate && !(FAR && p.gate_columns)) inv[t] *= activate(gate_logit(p, qi, h, 0), BITNET_HIP_ACT_SIGMOID);
         uint16_t *dst = out + (size_t)qi * ldo + (size_t)h * vdimp + g * 4;
 #pragma unroll
         for (int v = 0; v < NV; ++v)
             if (v * 16 < vdimp) {
-                f32x4 q = o[v][t] * (inv[t] * gate[t]);
+                f32x4 q = o[v][t] * inv[t];
                 if (FAR && p.gate_columns)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) q[i] *= activate(gate_logit(p, qi, h, v * 16 + g * 4 + i), BITNET_HIP_ACT_SIGMOID);
@@ -876,37 +909,91 @@ __global__ __launch_bounds__(256 * G, NV > 8 || NK > 2 ? 1 : 2) void k_kv8_prefi
     }
 }
 
+// two maps whose keys find no room together: each by itself, put together from records
+static bool maps_apart(const Gqa &g) { return g.maps == 2 && (g.dimp > 128 || g.vdimp > 128); }
+bool kv8_prefill_wants_records(const Gqa &g) { return maps_apart(g); }
+
+// Waves that share a tile, groups of them that share the rows, and stretches of the keys.  us of a step of a walk (128 columns; other sizes keep the proportions): four waves 1.72, with two
+// such workgroups on a compute unit 2.4; two groups of four waves 2.44 for two tiles; eight waves (twice the rows) 1.98; heads of more than 128 columns 3.3, one workgroup on a compute unit.
+// A launch lasts as long as its longest walk, or as its share of all of them with what workgroups of unequal length leave idle (an eighth; more where few long ones share a compute
+// unit's time).  Records cost 5 us and their bytes, 0.23 ns for 132 floats.
+// us by this rule, and of the others whole: 20 heads on 5 of 128, prompts of 130 / 600 / 2000 / 4000 12.8 / 23.1 / 49.5 / 125 (eight waves 15.4 / 28.6 / 72 / 134, two groups 14.9 / 23.1 / 49.5
+// / 135); 32 on 8, 4000 153 (four waves 176, two groups 195); 509 behind 20011, 12 of two maps, eight waves in 5 stretches 141 (whole 356 and more), 30 behind 7970, 20 heads, 28 (153).
+struct Kv8Form {
+    int groups, waves, parts;
+};
+static Kv8Form prefill_form(const Gqa &g, int n_ctx, int nq, bool room) {
+    const int group = (int)(g.heads / g.kv_heads), maps = maps_apart(g) ? 1 : (int)g.maps, longest = n_ctx / 64 + 1 - (gqa_first(g, n_ctx - 1) >> 6);
+    const double shortest = (n_ctx - nq) / 64 + 1 - (gqa_first(g, n_ctx - nq) >> 6), record = 0.23e-3 * (kGqaRecHead + g.vdimp) / 132 * nq * g.heads * g.maps;
+    const bool wide = g.dimp > 128 || g.vdimp > 128;
+    Kv8Form best{1, 4, 1};
+    double least = 1e30;
+    for (const Kv8Form f : {Kv8Form{1, 4, 1}, Kv8Form{2, 4, 1}, Kv8Form{1, 8, 1}}) {
+        if ((wide && (f.groups == 2 || f.waves == 8)) || (f.groups == 2 && maps == 2 && g.dimp > 64)) continue;
+        const int rows = 32 * f.waves / maps;
+        const double workgroups = (double)g.kv_heads * ((nq * (size_t)group + rows - 1) / rows) * (maps_apart(g) ? 2 : 1);
+        for (int parts = 1; parts <= (room ? 32 : 1) && (parts == 1 || (2 * parts <= longest && workgroups * parts <= 512)); ++parts) {
+            const double at_once = workgroups * parts, stretch = ((longest + f.groups - 1) / f.groups + parts - 1) / parts, all = workgroups * 0.5 * (longest + shortest) / f.groups;
+            const double walk = parts > 1 && at_once > 256 ? 2 * stretch : stretch;  // (stretches are all long: two rounds of them)
+            double us;
+            if (wide)
+                us = 3.3 * std::max(walk, 1.12 * all / 256);
+            else if (f.groups == 2)
+                us = 2.0 + 2.44 * std::max(walk, 1.4 * all / 256);
+            else if (f.waves == 8)
+                us = 2.5 + 1.98 * std::max(walk, 1.12 * all / 256);
+            else
+                us = at_once <= 256 ? 1.72 * stretch : std::max((parts > 1 ? 2.4 : 1.9) * stretch, 2.4 * 1.12 * all / 512);
+            if (parts > 1) us += 5.0 + record * parts;
+            if (us < least) least = us, best = Kv8Form{f.groups, f.waves, parts};
+        }
+    }
+    return best;
+}
 size_t kv8_prefill_floats(const Gqa &g, int n_ctx, int nq) {
-    const int parts = gqa_prefill_parts(g, n_ctx, nq);
-    return parts > 1 ? (size_t)nq * g.heads * g.maps * parts * (kGqaRecHead + g.vdimp) : 0;
+    const int parts = prefill_form(g, n_ctx, nq, true).parts;
+    return parts > 1 || maps_apart(g) ? (size_t)nq * g.heads * g.maps * parts * (kGqaRecHead + g.vdimp) : 0;
 }
 
-template <int NK, int NV, int G>
-static hipError_t prefill_go(const Kv8 &c, const uint16_t *q, size_t ldq, int n_ctx, int nq, uint16_t *out, size_t ldo, float *records, hipStream_t s) {
+template <int NK, int NV, int G, int W>
+static hipError_t prefill_go(const Kv8 &c, const uint16_t *q, size_t ldq, int n_ctx, int nq, uint16_t *out, size_t ldo, float *records, int parts, hipStream_t s) {
     const Gqa &g = c.g;
-    const int rows = g.maps == 2 ? 64 : 128, n_qb = (nq + rows - 1) / rows, parts = records ? gqa_prefill_parts(g, n_ctx, nq) : 1;
-    if constexpr (G == 2)
-        if (parts == 1 && !two_groups(g, rows, n_ctx, nq)) return prefill_go<NK, NV, 1>(c, q, ldq, n_ctx, nq, out, ldo, nullptr, s);
-    const size_t tiles = (size_t)G * kv8_buffers(NK, NV, (int)g.maps) * kv8_tile_bytes(NK, NV, (int)g.maps), sums = G == 2 ? (size_t)4 * 2 * 64 * (NV * 16 + 8) : 0;
+    const bool apart = maps_apart(g);
+    const int maps = apart ? 1 : (int)g.maps, rows = 32 * W / maps, n_qb = (int)((nq * (g.heads / g.kv_heads) + rows - 1) / rows);
+    const size_t tiles = (size_t)2 * G * kv8_tile_bytes(NK, NV, maps), sums = G == 2 ? (size_t)W * 2 * 64 * (NV * 16 + 8) : 0;
     const size_t lds = tiles > sums ? tiles : sums;
-    auto fn = g.maps == 2 ? k_kv8_prefill<NK, NV, 2, false, G> : g.far_weight || g.gate_columns ? k_kv8_prefill<NK, NV, 1, true, G> : k_kv8_prefill<NK, NV, 1, false, G>;
+    auto fn = k_kv8_prefill<NK, NV, 1, false, G, W>;
+    if (g.far_weight || g.gate_columns) fn = k_kv8_prefill<NK, NV, 1, true, G, W>;
+    if constexpr (NK <= 2 && NV <= 8 && 2 * G * kv8_tile_bytes(NK, NV, 2) <= 163840)
+        if (maps == 2) fn = k_kv8_prefill<NK, NV, 2, false, G, W>;
     if (lds > 65536) {
         const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(fn), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
         if (e != hipSuccess) return e;
     }
-    hipLaunchKernelGGL(fn, dim3(8 * ((g.heads + 7) / 8) * n_qb, parts), dim3(256 * G), lds, s, c, q, ldq, n_ctx, nq, out, ldo, n_qb, parts > 1 ? records : nullptr);
+    const bool leaves = parts > 1 || apart;
+    hipLaunchKernelGGL(fn, dim3(g.kv_heads * n_qb, parts, apart ? 2 : 1), dim3(64 * W * G), lds, s, c, q, ldq, n_ctx, nq, out, ldo, n_qb, leaves ? records : nullptr);
     const hipError_t e = hipGetLastError();
-    return e != hipSuccess || parts == 1 ? e : launch_gqa_merge_parts(g, records, parts, nq, out, ldo, s);
+    return e != hipSuccess || !leaves ? e : launch_gqa_merge_parts(g, records, parts, nq, out, ldo, s);
 }
 
-// records: kv8_prefill_floats(g, n_ctx, nq) of them, or none where a block's keys stay together
+template <int NK, int NV>
+static hipError_t prefill_pick(const Kv8 &c, const uint16_t *q, size_t ldq, int n_ctx, int nq, uint16_t *out, size_t ldo, float *records, hipStream_t s) {
+    const Kv8Form f = prefill_form(c.g, n_ctx, nq, records != nullptr);
+    if constexpr (NV <= 8) {
+        if (f.groups == 2) return prefill_go<NK, NV, 2, 4>(c, q, ldq, n_ctx, nq, out, ldo, records, f.parts, s);
+        if (f.waves == 8) return prefill_go<NK, NV, 1, 8>(c, q, ldq, n_ctx, nq, out, ldo, records, f.parts, s);
+    }
+    return prefill_go<NK, NV, 1, 4>(c, q, ldq, n_ctx, nq, out, ldo, records, f.parts, s);
+}
+
+// records: kv8_prefill_floats(g, n_ctx, nq) of them, or none where a block's keys stay together (not with maps apart)
 hipError_t launch_kv8_prefill(const Kv8 &c, const uint16_t *q, size_t ldq, int n_ctx, int nq, uint16_t *out, size_t ldo, float *records, hipStream_t s) {
     const Gqa &g = c.g;
-    if (!gqa_supported((int)g.dimp, (int)g.vdimp)) return hipErrorInvalidValue;
-    if (g.dimp <= 64 && g.vdimp <= 64) return prefill_go<1, 4, 2>(c, q, ldq, n_ctx, nq, out, ldo, records, s);
-    if (g.dimp <= 64 && g.vdimp <= 128) return prefill_go<1, 8, 2>(c, q, ldq, n_ctx, nq, out, ldo, records, s);
-    if (g.dimp <= 128 && g.vdimp <= 128) return prefill_go<2, 8, 2>(c, q, ldq, n_ctx, nq, out, ldo, records, s);
-    return prefill_go<4, 16, 1>(c, q, ldq, n_ctx, nq, out, ldo, records, s);
+    if (!gqa_supported((int)g.dimp, (int)g.vdimp) || (maps_apart(g) && !records)) return hipErrorInvalidValue;
+    if (g.dimp <= 64 && g.vdimp <= 64) return prefill_pick<1, 4>(c, q, ldq, n_ctx, nq, out, ldo, records, s);
+    if (g.dimp <= 64 && g.vdimp <= 128) return prefill_pick<1, 8>(c, q, ldq, n_ctx, nq, out, ldo, records, s);
+    if (g.dimp <= 128 && g.vdimp <= 128) return prefill_pick<2, 8>(c, q, ldq, n_ctx, nq, out, ldo, records, s);
+    return prefill_pick<4, 16>(c, q, ldq, n_ctx, nq, out, ldo, records, s);
 }
 
 }  // namespace bitnet_hip

@@ -145,7 +145,8 @@ class Attention:
     def prompt(self, hip, q, n0, n1, split=True, out=None, stream=0):
         n, no = n1 - n0, self.heads * self.vdimp
         out = u.zeros_bf16(n, no) if out is None else out
-        size = hip.kv8_prefill_scratch_bytes(self.attn, n1, n) if split else 0
+        apart = self.maps == 2 and max(self.dimp, self.vdimp) > 128  # (which the call does not do without)
+        size = hip.kv8_prefill_scratch_bytes(self.attn, n1, n) if split or apart else 0
         scratch = u.zeros_f32(size // 4) if size else None
         hip.kv8_prefill_dev(self.attn, self.cache.ks, self.cache.vs, q, q.shape[1], n1, n, out, no, scratch, size, stream=stream)
         return out

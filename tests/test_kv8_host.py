@@ -52,6 +52,7 @@ def test_refusals(built):
         (lambda: hip.kv8_prefill_dev(g, 16, 16, 24, 128, 10, 10, 16, 128), "kv8_prefill: bad arguments"),
         (lambda: hip.kv8_prefill_dev(g, 16, 16, 16, 128, 10, 10, 16, 126), "kv8_prefill: bad arguments"),
         (lambda: hip.kv8_prefill_dev(gqa(capacity=4096), 16, 16, 16, 128, 4000, 10, 16, 128, 16, 16), "kv8_prefill: scratch of 16 bytes"),
+        (lambda: hip.kv8_prefill_dev(gqa(maps=2, dim=160, dimp=160), 16, 16, 16, 1280, 10, 10, 16, 128), "want scratch"),
         (lambda: hip.kv8_prefill_dev(wide, 16, 16, 16, 2048, 10, 10, 16, 2048), "kv8: head"),
     ]
     for i, (call, match) in enumerate(bad):

@@ -229,7 +229,9 @@ int bitnet_hip_kv8_rows_dev(const bitnet_hip_gqa *a, float *k_scale, float *v_sc
     if (int rc = check_kv8(a, k_scale, v_scale)) return rc;
     if (!q) ldq = ld;
     BH_REQUIRE((q || a->taps == 0) && (!q || q != rows) && ldq >= a->heads * a->maps * a->dimp, "kv8_rows: bad place of the queries");
-    BH_REQUIRE(rows && pos && n > 0 && n <= a->capacity && ld >= gqa_row(a), "kv8_rows: bad arguments");
+    BH_REQUIRE(rows && pos && n > 0 && n <= a->capacity && ld >= gqa_row(a) && (n == 1 || (ld % 8 == 0 && ldq % 8 == 0)) && (((uintptr_t)rows | (uintptr_t)q) & 15) == 0 &&
+                   (a->taps == 0 || (uintptr_t)a->conv % 16 == 0),
+               "kv8_rows: bad arguments");
     BH_REQUIRE((a->heads + a->kv_heads) * a->maps + a->kv_heads < 65536, "kv8_rows: too many heads");
     BH_CHECK_DIMS(n, ld);
     BH_CHECK_DIMS(n, ldq);

@@ -1,9 +1,8 @@
 // gqa.hpp -- what the attention of shared keys and values has in common whatever its caches hold (kernels_gqa.hip, kernels_kv8.hip): the keys that a
-// position sees, the records they are cut into, rotation, distance penalty, gates, convolutions and the rows of query and key heads.
+// position sees, the records they are cut into, rotation, distance penalty, gates and convolutions.
 #pragma once
 
 #include <algorithm>
-#include <cfloat>
 #include <type_traits>
 
 #include "dense.hpp"
@@ -61,19 +60,6 @@ __device__ __forceinline__ FarPenalty far_penalty(const Gqa &p, int h) {
     return f;
 }
 __device__ __forceinline__ float nearer(float score, const FarPenalty &f, int distance) { return fmaf(-f.weight, __log2f(fmaf(f.rate, (float)distance, 1.0f)), score); }
-// How a vector of an 8-bit cache is held: whole numbers -127 .. 127 and one scale.  The scale stays 32 bits wide.  What is smaller than 1.5e-36 throughout counts as zero (its scale would
-// have no full mantissa), and a vector with a value that is not finite has a scale that is not a number, so that whoever sees it gets NaN.
-struct Kv8Scale {
-    float scale, factor;
-};
-__device__ __forceinline__ Kv8Scale kv8_scale(float largest, bool finite) {
-    if (!finite) return {__builtin_nanf(""), 0.f};
-    if (!(largest >= 1.5e-36f)) return {0.f, 0.f};
-    return {largest / 127.0f, 127.0f / largest};
-}
-__device__ __forceinline__ int kv8_number(float v, const Kv8Scale &s) { return s.factor == 0.f ? 0 : (int)rintf(v * s.factor); }
-__device__ __forceinline__ bool is_finite(float v) { return fabsf(v) <= FLT_MAX; }
-
 // columns of a row of projections that a convolution covers
 __host__ __device__ __forceinline__ int gqa_channels(const Gqa &p) {
     if (p.queries_only) return (int)(p.heads * p.maps * p.dimp);
@@ -85,130 +71,6 @@ __device__ __forceinline__ float raw_value(const Gqa &p, const TR *rows, size_t 
     if (t >= 0) return ld_act(rows + (size_t)t * ld, c);
     const int at = pos0 + t;
     return at >= 0 ? p.ring[(size_t)(at % (int)p.taps) * channels + c] : 0.f;
-}
-
-constexpr int kRowTokens = 16, kRowCols = 32;
-
-// Four tokens of a query or key head of up to 128 NJ columns: a lane holds neighbouring elements, so that a pair turns within it.  TAPS: those of the convolution
-// (0: none, -1: any number).  TC int8_t: a key's numbers, and its scale by position in `scales`.
-template <class TR, class TC, int NJ, int TAPS>
-__device__ __forceinline__ void head_rows(const Gqa &p, const TR *rows, size_t ld, int pos0, int t0, int n, int y, bool key, TC *cache, TR *queries, size_t ldq, float *scales = nullptr) {
-    constexpr int U = kRowTokens / 4;
-    constexpr bool CONV = TAPS != 0;
-    const int lane = threadIdx.x & 63, dim = (int)p.dim, dimp = (int)p.dimp, turned = (int)p.rot_dims, half = turned >> 1;
-    const float *w = key ? p.k_weight : p.q_weight;
-    float v[U][NJ][2], cs[U][NJ], sn[U][NJ], factor[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const int t = min(t0 + u, n - 1);
-        const TR *row = rows + (size_t)t * ld + (size_t)y * dimp;
-        factor[u] = key ? 1.0f : p.q_factor[pos0 + t];
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-            const int i = min(2 * lane + 128 * j, dimp - 2);
-            if (CONV)
-                v[u][j][0] = v[u][j][1] = 0.f;
-            else
-                v[u][j][0] = ld_act(row, i), v[u][j][1] = ld_act(row, i + 1);
-            cs[u][j] = 1.0f, sn[u][j] = 0.f;
-            if (turned && 2 * lane + 128 * j < turned) {
-                const size_t at = (size_t)(pos0 + t) * half + lane + 64 * j;
-                cs[u][j] = p.rope_cos[at], sn[u][j] = p.rope_sin[at];
-            }
-        }
-    }
-    if (TAPS > 0) {  // the tokens and those ahead of them once, in registers
-        constexpr int T = TAPS > 0 ? TAPS : 1;
-        const int channels = gqa_channels(p);
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-            const int c = y * dimp + min(2 * lane + 128 * j, dimp - 2);
-            float f[T][2], raw[U + T - 1][2];
-#pragma unroll
-            for (int k = 0; k < T; ++k) f[k][0] = p.conv[(size_t)k * channels + c], f[k][1] = p.conv[(size_t)k * channels + c + 1];
-            if (t0 >= T - 1) {
-#pragma unroll
-                for (int k = 0; k < U + T - 1; ++k) {
-                    const TR *row = rows + (size_t)min(t0 - (T - 1) + k, n - 1) * ld;
-                    raw[k][0] = ld_act(row, c), raw[k][1] = ld_act(row, c + 1);
-                }
-            } else {
-#pragma unroll
-                for (int k = 0; k < U + T - 1; ++k) {
-                    const int t = min(t0 - (T - 1) + k, n - 1);
-                    raw[k][0] = raw_value(p, rows, ld, pos0, t, c, channels), raw[k][1] = raw_value(p, rows, ld, pos0, t, c + 1, channels);
-                }
-            }
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-#pragma unroll
-                for (int k = 0; k < T; ++k) v[u][j][0] += f[k][0] * raw[u + k][0], v[u][j][1] += f[k][1] * raw[u + k][1];
-        }
-    } else if (CONV) {
-        const int taps = (int)p.taps, channels = gqa_channels(p);
-        for (int k = 0; k < taps; ++k)
-#pragma unroll
-            for (int j = 0; j < NJ; ++j) {
-                const int c = y * dimp + min(2 * lane + 128 * j, dimp - 2);
-                const float f0 = p.conv[(size_t)k * channels + c], f1 = p.conv[(size_t)k * channels + c + 1];
-#pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    const int t = min(t0 + u, n - 1) - (taps - 1) + k;
-                    v[u][j][0] += f0 * raw_value(p, rows, ld, pos0, t, c, channels), v[u][j][1] += f1 * raw_value(p, rows, ld, pos0, t, c + 1, channels);
-                }
-            }
-    }
-    float wv[NJ][2];
-#pragma unroll
-    for (int j = 0; j < NJ; ++j)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) wv[j][e] = w && 2 * lane + 128 * j + e < dim ? w[2 * lane + 128 * j + e] : 1.0f;  // (padding columns hold zeros)
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-        if (w || p.unit_norm) {
-            float ss = 0.f;
-#pragma unroll
-            for (int j = 0; j < NJ; ++j) ss += 2 * lane + 128 * j < dimp ? v[u][j][0] * v[u][j][0] + v[u][j][1] * v[u][j][1] : 0.f;
-            factor[u] *= 1.0f / sqrtf(wave_sum(ss) / (float)dim + p.eps);
-        }
-        if (t0 + u >= n) continue;
-        TR *row = queries + (size_t)(t0 + u) * ldq + (size_t)y * dimp;
-        if constexpr (std::is_same_v<TC, int8_t>) {
-            if (key) {
-                float x[NJ][2], largest = 0.f;
-                bool finite = true;
-#pragma unroll
-                for (int j = 0; j < NJ; ++j) {
-                    const float a = v[u][j][0] * factor[u] * wv[j][0], b = v[u][j][1] * factor[u] * wv[j][1];
-                    x[j][0] = a * cs[u][j] - b * sn[u][j], x[j][1] = b * cs[u][j] + a * sn[u][j];
-                    if (2 * lane + 128 * j < dimp) largest = fmaxf(largest, fmaxf(fabsf(x[j][0]), fabsf(x[j][1]))), finite = finite && is_finite(x[j][0]) && is_finite(x[j][1]);
-                }
-                const Kv8Scale s = kv8_scale(rows_max(row_max(largest)), __all(finite));
-                int8_t *dst = cache + (size_t)(pos0 + t0 + u) * dimp;
-#pragma unroll
-                for (int j = 0; j < NJ; ++j)
-                    if (2 * lane + 128 * j < dimp)
-                        *reinterpret_cast<uint16_t *>(dst + 2 * lane + 128 * j) = (uint16_t)((kv8_number(x[j][0], s) & 0xff) | (kv8_number(x[j][1], s) & 0xff) << 8);
-                if (lane == 0) scales[pos0 + t0 + u] = s.scale;
-                continue;
-            }
-        }
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-            const int i = 2 * lane + 128 * j;
-            if (i >= dimp) continue;
-            const float a = v[u][j][0] * factor[u] * wv[j][0], b = v[u][j][1] * factor[u] * wv[j][1];
-            const float x = a * cs[u][j] - b * sn[u][j], z = b * cs[u][j] + a * sn[u][j];
-            if constexpr (!std::is_same_v<TC, int8_t>) {
-                if (key) {
-                    TC *dst = cache + (size_t)(pos0 + t0 + u) * dimp;
-                    st_act(dst, i, x), st_act(dst, i + 1, z);
-                    continue;
-                }
-            }
-            st_act(row, i, x), st_act(row, i + 1, z);
-        }
-    }
 }
 
 // ---- how a prompt's launch is shared out -----------------------------------------------------------------------------

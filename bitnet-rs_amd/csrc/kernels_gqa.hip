@@ -21,6 +21,108 @@ bool gqa_supported(int dimp, int vdimp) { return dimp <= 256 && vdimp <= 256; }
 // ---- rows of projections ----------------------------------------------------------------------------------------------
 // blockIdx.y: query heads x maps, key heads x maps (sixteen tokens per workgroup, four per wave), then value heads in groups of 32 columns (64
 // tokens, every fourth workgroup).
+constexpr int kRowTokens = 16, kRowCols = 32;
+
+// Four tokens of a query or key head of up to 128 NJ columns: a lane holds neighbouring elements, so that a pair turns within it.  TAPS: those of the convolution
+// (0: none, -1: any number).
+template <class TR, class TC, int NJ, int TAPS>
+__device__ __forceinline__ void head_rows(const Gqa &p, const TR *rows, size_t ld, int pos0, int t0, int n, int y, bool key, TC *cache, TR *queries, size_t ldq) {
+    constexpr int U = kRowTokens / 4;
+    constexpr bool CONV = TAPS != 0;
+    const int lane = threadIdx.x & 63, dim = (int)p.dim, dimp = (int)p.dimp, turned = (int)p.rot_dims, half = turned >> 1;
+    const float *w = key ? p.k_weight : p.q_weight;
+    float v[U][NJ][2], cs[U][NJ], sn[U][NJ], factor[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int t = min(t0 + u, n - 1);
+        const TR *row = rows + (size_t)t * ld + (size_t)y * dimp;
+        factor[u] = key ? 1.0f : p.q_factor[pos0 + t];
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            const int i = min(2 * lane + 128 * j, dimp - 2);
+            if (CONV)
+                v[u][j][0] = v[u][j][1] = 0.f;
+            else
+                v[u][j][0] = ld_act(row, i), v[u][j][1] = ld_act(row, i + 1);
+            cs[u][j] = 1.0f, sn[u][j] = 0.f;
+            if (turned && 2 * lane + 128 * j < turned) {
+                const size_t at = (size_t)(pos0 + t) * half + lane + 64 * j;
+                cs[u][j] = p.rope_cos[at], sn[u][j] = p.rope_sin[at];
+            }
+        }
+    }
+    if (TAPS > 0) {  // the tokens and those ahead of them once, in registers
+        constexpr int T = TAPS > 0 ? TAPS : 1;
+        const int channels = gqa_channels(p);
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            const int c = y * dimp + min(2 * lane + 128 * j, dimp - 2);
+            float f[T][2], raw[U + T - 1][2];
+#pragma unroll
+            for (int k = 0; k < T; ++k) f[k][0] = p.conv[(size_t)k * channels + c], f[k][1] = p.conv[(size_t)k * channels + c + 1];
+            if (t0 >= T - 1) {
+#pragma unroll
+                for (int k = 0; k < U + T - 1; ++k) {
+                    const TR *row = rows + (size_t)min(t0 - (T - 1) + k, n - 1) * ld;
+                    raw[k][0] = ld_act(row, c), raw[k][1] = ld_act(row, c + 1);
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < U + T - 1; ++k) {
+                    const int t = min(t0 - (T - 1) + k, n - 1);
+                    raw[k][0] = raw_value(p, rows, ld, pos0, t, c, channels), raw[k][1] = raw_value(p, rows, ld, pos0, t, c + 1, channels);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int k = 0; k < T; ++k) v[u][j][0] += f[k][0] * raw[u + k][0], v[u][j][1] += f[k][1] * raw[u + k][1];
+        }
+    } else if (CONV) {
+        const int taps = (int)p.taps, channels = gqa_channels(p);
+        for (int k = 0; k < taps; ++k)
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                const int c = y * dimp + min(2 * lane + 128 * j, dimp - 2);
+                const float f0 = p.conv[(size_t)k * channels + c], f1 = p.conv[(size_t)k * channels + c + 1];
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const int t = min(t0 + u, n - 1) - (taps - 1) + k;
+                    v[u][j][0] += f0 * raw_value(p, rows, ld, pos0, t, c, channels), v[u][j][1] += f1 * raw_value(p, rows, ld, pos0, t, c + 1, channels);
+                }
+            }
+    }
+    float wv[NJ][2];
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) wv[j][e] = w && 2 * lane + 128 * j + e < dim ? w[2 * lane + 128 * j + e] : 1.0f;  // (padding columns hold zeros)
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        if (w || p.unit_norm) {
+            float ss = 0.f;
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) ss += 2 * lane + 128 * j < dimp ? v[u][j][0] * v[u][j][0] + v[u][j][1] * v[u][j][1] : 0.f;
+            factor[u] *= 1.0f / sqrtf(wave_sum(ss) / (float)dim + p.eps);
+        }
+        if (t0 + u >= n) continue;
+        TR *row = queries + (size_t)(t0 + u) * ldq + (size_t)y * dimp;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            const int i = 2 * lane + 128 * j;
+            if (i >= dimp) continue;
+            const float a = v[u][j][0] * factor[u] * wv[j][0], b = v[u][j][1] * factor[u] * wv[j][1];
+            const float x = a * cs[u][j] - b * sn[u][j], z = b * cs[u][j] + a * sn[u][j];
+            if (key) {
+                TC *dst = cache + (size_t)(pos0 + t0 + u) * dimp;
+                st_act(dst, i, x), st_act(dst, i + 1, z);
+            } else {
+                st_act(row, i, x), st_act(row, i + 1, z);
+            }
+        }
+    }
+}
+
 // TAPS (as head_rows): every column passes a convolution over time first, and the queries go to a place of their own
 template <class TR, class TC, int NJ, int TAPS>
 __global__ __launch_bounds__(256) void k_gqa_rows(Gqa p, const TR *rows, size_t ld, const int *pos_ptr, int n, TR *queries, size_t ldq) {

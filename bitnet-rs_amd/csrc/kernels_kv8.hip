@@ -1,6 +1,6 @@
 // kernels_kv8.hip -- the attention of kernels_gqa.hip over caches of 8 bits (gfx950).
 //
-// A head's key (of one map) and a head's value at a position are whole numbers -127 .. 127 with one f32 scale each: value = number * scale (kv8_scale, gqa.hpp).  One scale
+// A head's key (of one map) and a head's value at a position are whole numbers -127 .. 127 with one f32 scale each: value = number * scale (kv8_scale).  One scale
 // per position, not per block of them: an append touches nothing that is written, and the cache is a function of the tokens alone, however they came in.
 // Keys int8 [kv head][map][capacity][dimp]; values int8 [kv head][capacity / 32][vdimp / 32][16][4][2][8]: column c at position p lies at [p / 32][c / 32][c % 16]
 // [p % 32 / 8][c % 32 / 16][p % 8], so that 32 keys by 32 columns are 1 KiB in the order in which the matrix cores take them, and 32 keys of a head are one piece.
@@ -11,6 +11,8 @@
 // A step's scores are whole: a query is cut into three balanced digits of 8 bits with one scale (23 bits), the products with the keys' numbers are exact in 32-bit integers, and
 // the scales come behind them; a weight times its value's scale meets the values' numbers, which f16 holds exactly, as a (high, low) pair of f16.  A prompt's queries are bf16 and
 // so are its outputs: f16 throughout (see there).
+#include <cfloat>
+
 #include "gqa.hpp"
 
 namespace bitnet_hip {
@@ -52,87 +54,286 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 __device__ __forceinline__ int exponent_above(float v) { return v > 0.f ? max(__builtin_amdgcn_frexp_expf(v), -100) : -100; }
 __device__ __forceinline__ float power2(int e) { return __builtin_amdgcn_ldexpf(1.0f, e); }
 
+// How a vector of an 8-bit cache is held: whole numbers -127 .. 127 and one scale.  The scale stays 32 bits wide.  What is smaller than 1.5e-36 throughout counts as zero (its scale would
+// have no full mantissa), and a vector with a value that is not finite has a scale that is not a number, so that whoever sees it gets NaN.
+struct Kv8Scale {
+    float scale, factor;
+};
+__device__ __forceinline__ Kv8Scale kv8_scale(float largest, bool finite) {
+    if (!finite) return {__builtin_nanf(""), 0.f};
+    if (!(largest >= 1.5e-36f)) return {0.f, 0.f};
+    return {largest / 127.0f, 127.0f / largest};
+}
+__device__ __forceinline__ int kv8_number(float v, const Kv8Scale &s) { return s.factor == 0.f ? 0 : (int)rintf(v * s.factor); }
+__device__ __forceinline__ bool is_finite(float v) { return fabsf(v) <= FLT_MAX; }
+
 // where column c of a kv head's values at position pos lies
 __device__ __forceinline__ size_t kv8_value_at(int vdimp, int pos, int c) {
     return (size_t)(pos >> 5) * (vdimp * 32) + (c >> 5) * 1024 + (c & 15) * 64 + (pos >> 3 & 3) * 16 + (c >> 4 & 1) * 8 + (pos & 7);
 }
 
 // ---- rows of projections ----------------------------------------------------------------------------------------------
-// blockIdx.y: query heads x maps and key heads x maps (sixteen tokens per workgroup), then value heads: 32 positions of whole tiles, eight threads a token.
-template <class TR, int NJ, int TAPS>
-__global__ __launch_bounds__(256) void k_kv8_rows(Kv8 c, const TR *rows, size_t ld, const int *pos_ptr, int n, TR *queries, size_t ldq) {
-    __shared__ __attribute__((aligned(16))) uint8_t tile[256 * 32];
+// Bound by memory: 16384 tokens of 20 heads on 5 of 128 columns, bf16, half of them turned, are 232 MB in 50-52 us (4.5 TB/s; a copy reaches 5.3).  By heads first and pairs of columns it
+// was 80, whole rows at a time 64; a wave's heads in turn, with the rotation and the next columns in registers, took the rest.  One token 4.0, 1531 of two maps of 64 / 128 8.7.
+// A lane holds eight neighbouring columns, KL or VL lanes a head's row: pairs turn within a lane, and a wave takes 64 / KL tokens at a time, R times.  Workgroups: four waves'
+// tokens and a part of the heads (query heads x maps, key heads x maps; one after the other, the next one's columns on their way), then values, a wave a tile of 32 positions, its rows through LDS into the cache's order.
+
+template <int L>
+__device__ __forceinline__ float lanes_max(float v) {
+    v = fmaxf(v, dpp<0xb1>(v));   // quad_perm [1,0,3,2]
+    v = fmaxf(v, dpp<0x4e>(v));   // quad_perm [2,3,0,1]
+    v = fmaxf(v, dpp<0x141>(v));  // row_half_mirror
+    if (L >= 16) v = fmaxf(v, dpp<0x140>(v));  // row_mirror
+    if (L >= 32) {
+        float w = v;
+        swap_rows16(v, w);
+        v = fmaxf(v, w);
+    }
+    return v;
+}
+template <int L>
+__device__ __forceinline__ float lanes_sum(float v) {
+    v += dpp<0xb1>(v);
+    v += dpp<0x4e>(v);
+    v += dpp<0x141>(v);
+    if (L >= 16) v += dpp<0x140>(v);
+    if (L >= 32) {
+        float w = v;
+        swap_rows16(v, w);
+        v += w;
+    }
+    return v;
+}
+struct Eight {
+    float v[8];
+};
+__device__ __forceinline__ Eight load8(const float *p) {
+    const f32x4 a = *reinterpret_cast<const f32x4 *>(p), b = *reinterpret_cast<const f32x4 *>(p + 4);
+    return {{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}};
+}
+__device__ __forceinline__ Eight load8(const uint16_t *p) {
+    const u32x4 a = *reinterpret_cast<const u32x4 *>(p);
+    Eight r;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r.v[i] = bf2f(a[i >> 1] >> (16 * (i & 1)) & 0xffffu);
+    return r;
+}
+__device__ __forceinline__ void store8(float *p, const Eight &x) {
+    *reinterpret_cast<f32x4 *>(p) = f32x4{x.v[0], x.v[1], x.v[2], x.v[3]};
+    *reinterpret_cast<f32x4 *>(p + 4) = f32x4{x.v[4], x.v[5], x.v[6], x.v[7]};
+}
+__device__ __forceinline__ void store8(uint16_t *p, const Eight &x) {
+    bf16x8 b;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) b[i] = (__bf16)x.v[i];
+    *reinterpret_cast<bf16x8 *>(p) = b;
+}
+// eight columns of the row of projections t from column c on, convolved
+template <class TR, int TAPS>
+__device__ __forceinline__ Eight row8(const Gqa &p, const TR *rows, size_t ld, int pos0, int t, int c, int channels) {
+    if (TAPS == 0) return load8(rows + (size_t)t * ld + c);
+    Eight r{};
+    const int taps = TAPS > 0 ? TAPS : (int)p.taps;
+#pragma unroll TAPS > 0 ? TAPS : 1
+    for (int k = 0; k < taps; ++k) {
+        const int at = t - (taps - 1) + k;
+        const Eight f = load8(p.conv + (size_t)k * channels + c);
+        Eight x;
+        if (at >= 0)
+            x = load8(rows + (size_t)at * ld + c);
+        else
+            for (int i = 0; i < 8; ++i) x.v[i] = raw_value(p, rows, ld, pos0, at, c + i, channels);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) r.v[i] = fmaf(f.v[i], x.v[i], r.v[i]);
+    }
+    return r;
+}
+// the lane's eight numbers of a vector that L lanes share
+template <int L>
+__device__ __forceinline__ Kv8Scale eight_numbers(const Eight &x, bool live, u32x2 &numbers) {
+    float largest = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) largest = fmaxf(largest, live ? (is_finite(x.v[i]) ? fabsf(x.v[i]) : INFINITY) : 0.f);
+    largest = lanes_max<L>(largest);
+    const Kv8Scale s = kv8_scale(largest, is_finite(largest));
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        uint32_t w = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w |= (uint32_t)(kv8_number(x.v[4 * h + i], s) & 0xff) << (8 * i);
+        numbers[h] = w;
+    }
+    return s;
+}
+
+template <class TR, int KL, int VL, int TAPS, int R>
+__global__ __launch_bounds__(256) void k_kv8_rows(Kv8 c, const TR *rows, size_t ld, const int *pos_ptr, int n, TR *queries, size_t ldq, int blocks, int chunks) {
+    constexpr int PITCH = VL * 8 + 4;
+    __shared__ uint32_t turned_round[4][32][PITCH / 4];
     const Gqa &p = c.g;
-    const int tid = threadIdx.x, wave = tid >> 6, pos0 = *pos_ptr;
-    const int nq = (int)(p.heads * p.maps), nk = (int)(p.kv_heads * p.maps), dimp = (int)p.dimp, vdimp = (int)p.vdimp, y = blockIdx.y;
-    if (y < nq + nk) {
-        const bool key = y >= nq;
-        const int t0 = blockIdx.x * kRowTokens + wave * (kRowTokens / 4);
-        if (t0 >= n) return;
-        int8_t *cache = key ? (int8_t *)p.kcache + (size_t)(y - nq) * p.capacity * dimp : nullptr;
-        head_rows<TR, int8_t, NJ, TAPS>(p, rows, ld, pos0, t0, n, y, key, cache, queries, ldq, key ? c.k_scale + (size_t)(y - nq) * p.capacity : nullptr);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), pos0 = *pos_ptr, channels = gqa_channels(p);
+    const int nq = (int)(p.heads * p.maps), nk = (int)(p.kv_heads * p.maps), dim = (int)p.dim, dimp = (int)p.dimp, vdimp = (int)p.vdimp, heads = p.queries_only ? nq : nq + nk;
+    if ((int)blockIdx.x < blocks * chunks) {
+        constexpr int AT_ONCE = 64 / KL;
+        // (the wave's first token is one for all lanes: places are its own and 32 bits for the lane)
+        const int block = blockIdx.x / chunks, chunk = blockIdx.x - block * chunks, h0 = heads * chunk / chunks, h1 = heads * (chunk + 1) / chunks;
+        const int col = lane % KL * 8, half = (int)p.rot_dims >> 1, first = (block * 4 + wave) * AT_ONCE * R, left = n - 1 - first, mine = lane / KL;
+        const bool live = col < dimp, fours = half % 4 == 0 && (((uintptr_t)p.rope_cos | (uintptr_t)p.rope_sin) & 15) == 0;
+        const int at = min(col, dimp - 8);
+        if (left < 0) return;
+        const TR *src = rows + (size_t)first * ld;
+        const float per_dim = 1.0f / (float)dim, *ct = p.rope_cos + (size_t)(pos0 + first) * half, *st = p.rope_sin + (size_t)(pos0 + first) * half, *fac = p.q_factor + pos0 + first;
+        Eight x[R], next[R], wv;
+        auto fetch = [&](int y) {
+#pragma unroll
+            for (int u = 0; u < R; ++u) {
+                const int t = min(mine + u * AT_ONCE, left);
+                if (TAPS == 0)
+                    next[u] = load8(src + (unsigned)(t * (int)ld + y * dimp + at));
+                else
+                    next[u] = row8<TR, TAPS>(p, rows, ld, pos0, first + t, y * dimp + at, channels);
+            }
+        };
+        auto weights = [&](const float *w) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) wv.v[i] = w && at + i < dim ? w[at + i] : 1.0f;
+        };
+        fetch(h0);
+        weights(h0 < nq ? p.q_weight : p.k_weight);
+        f32x4 cs[R], sn[R];
+        float factor[R];
+#pragma unroll
+        for (int u = 0; u < R; ++u) {
+            const int t = min(mine + u * AT_ONCE, left);
+            factor[u] = fac[(unsigned)t];
+            if (half) {
+                if (fours) {
+                    const int pair = t * half + min(at >> 1, half - 4);
+                    cs[u] = *reinterpret_cast<const f32x4 *>(ct + (unsigned)pair), sn[u] = *reinterpret_cast<const f32x4 *>(st + (unsigned)pair);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) cs[u][e] = ct[(unsigned)(t * half + min((at >> 1) + e, half - 1))], sn[u][e] = st[(unsigned)(t * half + min((at >> 1) + e, half - 1))];
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e)  // (pairs past the turned ones: by nothing)
+                    if ((at >> 1) + e >= half) cs[u][e] = 1.0f, sn[u][e] = 0.f;
+            }
+        }
+        for (int y = h0; y < h1; ++y) {
+            const bool key = y >= nq;
+#pragma unroll
+            for (int u = 0; u < R; ++u) x[u] = next[u];
+            if (y == nq && y > h0) weights(p.k_weight);
+            if (y + 1 < h1) fetch(y + 1);
+            TR *out = queries + (size_t)first * ldq + (size_t)y * dimp;
+            const size_t row0 = (size_t)(y - nq) * p.capacity + pos0 + first;  // (keys)
+            int8_t *cache = (int8_t *)p.kcache + row0 * dimp;
+            float *scales = c.k_scale + row0;
+#pragma unroll
+            for (int u = 0; u < R; ++u) {
+                const int t = mine + u * AT_ONCE;
+                float f = key ? 1.0f : factor[u];
+                if ((key ? p.k_weight : p.q_weight) || p.unit_norm) {
+                    float ss = 0.f;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) ss = fmaf(x[u].v[i], x[u].v[i], ss);
+                    f *= __builtin_amdgcn_rsqf(fmaf(lanes_sum<KL>(live ? ss : 0.f), per_dim, p.eps));  // (off by a unit in the last place at most)
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[u].v[i] *= f * wv.v[i];
+                if (half)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float a = x[u].v[2 * e], b = x[u].v[2 * e + 1];
+                        x[u].v[2 * e] = a * cs[u][e] - b * sn[u][e], x[u].v[2 * e + 1] = b * cs[u][e] + a * sn[u][e];
+                    }
+                if (!key) {
+                    if (live && t <= left) store8(out + (unsigned)(t * (int)ldq + col), x[u]);
+                    continue;
+                }
+                u32x2 numbers;
+                const Kv8Scale s = eight_numbers<KL>(x[u], live, numbers);
+                if (live && t <= left) *reinterpret_cast<u32x2 *>(cache + (unsigned)(t * dimp + col)) = numbers;
+                if (col == 0 && t <= left) scales[(unsigned)t] = s.scale;
+            }
+        }
         return;
     }
-    const int kv = y - nq - nk, first = ((pos0 >> 5) + (int)blockIdx.x) * 32;
-    if (first >= pos0 + n) return;
-    const int at = tid >> 3, part = tid & 7, t = first + at - pos0, column = (p.values_are_keys ? nq : nq + nk) * dimp + kv * vdimp;
-    const bool live = t >= 0 && t < n;
-    const int taps = TAPS > 0 ? TAPS : TAPS < 0 ? (int)p.taps : 1, channels = gqa_channels(p);
-    f32x4 v[8];
-    float largest = 0.f;
-    bool finite = true;
+    constexpr int AT_ONCE = 64 / VL, ROUNDS = 32 / AT_ONCE;
+    const int at_block = (int)blockIdx.x - blocks * chunks, block = at_block / (int)p.kv_heads, kv = at_block - block * (int)p.kv_heads, tile = ((pos0 >> 5) + block * 4 + wave) * 32, col = lane % VL * 8, column = (p.values_are_keys ? nq : nq + nk) * dimp + kv * vdimp;
+    const bool live = col < vdimp;
+    const int at = min(col, vdimp - 8);
+    if (tile < pos0 + n) {
+        Eight x[ROUNDS];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        v[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-        if (!live || 32 * j >= vdimp) continue;
-        const int at_col = column + 32 * j + 4 * part;
+        for (int u = 0; u < ROUNDS; ++u) x[u] = row8<TR, TAPS>(p, rows, ld, pos0, min(max(tile + u * AT_ONCE + lane / VL - pos0, 0), n - 1), column + at, channels);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            if (TAPS != 0)
-                for (int k = 0; k < taps; ++k) v[j][e] += p.conv[(size_t)k * channels + at_col + e] * raw_value(p, rows, ld, pos0, t - (taps - 1) + k, at_col + e, channels);
-            else
-                v[j][e] = ld_act(rows + (size_t)t * ld, at_col + e);
-            largest = fmaxf(largest, fabsf(v[j][e])), finite = finite && is_finite(v[j][e]);
+        for (int u = 0; u < ROUNDS; ++u) {
+            const int row = u * AT_ONCE + lane / VL, t = tile + row - pos0;
+            if (tile + (u + 1) * AT_ONCE <= pos0 || tile + u * AT_ONCE >= pos0 + n) continue;  // (no token of these)
+            u32x2 numbers;
+            const Kv8Scale s = eight_numbers<VL>(x[u], live, numbers);
+            if (col == 0 && t >= 0 && t < n) c.v_scale[(size_t)kv * p.capacity + tile + row] = s.scale;
+            turned_round[wave][row][(col >> 2)] = numbers.x, turned_round[wave][row][(col >> 2) + 1] = numbers.y;
         }
     }
-    if (!finite) largest = INFINITY;  // (no finite value is)
-#pragma unroll
-    for (int d = 1; d < 8; d *= 2) largest = fmaxf(largest, __shfl_xor(largest, d, 64));
-    const Kv8Scale s = kv8_scale(largest, is_finite(largest));
-    if (live && part == 0) c.v_scale[(size_t)kv * p.capacity + first + at] = s.scale;
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-        if (32 * j < vdimp)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) tile[kv8_value_at(vdimp, at, 32 * j + 4 * part + e)] = (uint8_t)kv8_number(v[j][e], s);
     __syncthreads();
-    uint8_t *dst = (uint8_t *)p.vcache + (size_t)kv * vdimp * p.capacity + (size_t)first * vdimp;
-    for (int i = tid; i < vdimp * 2; i += 256) {  // sixteen bytes: eight positions of two columns
-        const int t8 = first + (i & 3) * 8 - pos0;
+    if (tile >= pos0 + n) return;
+    uint8_t *dst = (uint8_t *)p.vcache + (size_t)kv * vdimp * p.capacity + (size_t)tile * vdimp;
+    // four columns and the four 16 further on, eight positions: two blocks of four by four bytes each, turned
+    for (int i = lane; i < vdimp >> 1; i += 64) {
+        const int p8 = (i & 3) * 8, c4 = i >> 2 & 3, c32 = i >> 4, t8 = tile + p8 - pos0;
+        uint32_t out[4][4];  // [column][16 bytes: eight positions of it, eight of the one 16 further on]
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                uint32_t a[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) a[e] = turned_round[wave][p8 + 4 * q + e][c32 * 8 + h * 4 + c4];
+                const uint32_t l0 = __builtin_amdgcn_perm(a[1], a[0], 0x05010400u), l1 = __builtin_amdgcn_perm(a[3], a[2], 0x05010400u);  // (columns 0 and 1 of two positions)
+                const uint32_t h0 = __builtin_amdgcn_perm(a[1], a[0], 0x07030602u), h1 = __builtin_amdgcn_perm(a[3], a[2], 0x07030602u);  // (2 and 3)
+                out[0][2 * h + q] = __builtin_amdgcn_perm(l1, l0, 0x05040100u), out[1][2 * h + q] = __builtin_amdgcn_perm(l1, l0, 0x07060302u);
+                out[2][2 * h + q] = __builtin_amdgcn_perm(h1, h0, 0x05040100u), out[3][2 * h + q] = __builtin_amdgcn_perm(h1, h0, 0x07060302u);
+            }
+        uint8_t *to = dst + (c32 * 16 + c4 * 4) * 64 + (i & 3) * 16;
         if (t8 >= 0 && t8 + 8 <= n) {
-            *reinterpret_cast<u32x4 *>(dst + i * 16) = *reinterpret_cast<const u32x4 *>(tile + i * 16);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) *reinterpret_cast<u32x4 *>(to + e * 64) = u32x4{out[e][0], out[e][1], out[e][2], out[e][3]};
         } else {
-            for (int e = 0; e < 16; ++e)
-                if (t8 + (e & 7) >= 0 && t8 + (e & 7) < n) dst[i * 16 + e] = tile[i * 16 + e];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (int k = 0; k < 16; ++k)
+                    if (t8 + (k & 7) >= 0 && t8 + (k & 7) < n) to[e * 64 + k] = (uint8_t)(out[e][k >> 2] >> (8 * (k & 3)));
         }
     }
 }
 
-template <class TR>
-static hipError_t rows_go(const Kv8 &c, const void *rows, size_t ld, const int *pos, int n, void *q, size_t ldq, hipStream_t s) {
+template <class TR, int KL, int VL, int TAPS>
+static hipError_t rows_launch(const Kv8 &c, const void *rows, size_t ld, const int *pos, int n, void *q, size_t ldq, hipStream_t s) {
     const Gqa &g = c.g;
-    const int keys = g.queries_only ? 0 : (int)(g.kv_heads * g.maps + g.kv_heads);
+    const int heads = (int)(g.heads * g.maps + (g.queries_only ? 0 : g.kv_heads * g.maps)), at_once = 4 * 64 / KL;
+    const bool few = n <= at_once;  // (a wave takes its tokens at once, else four times as many in turn)
+    const int each = few ? at_once : 4 * at_once, blocks = (n + each - 1) / each;
     // (n tokens from anywhere in a tile of 32 on reach into (n + 62) / 32 of them at most)
-    const dim3 grid(std::max((n + kRowTokens - 1) / kRowTokens, (n + 62) / 32), (int)(g.heads * g.maps) + keys);
-    auto pick = [&](auto narrow, auto wide) { return g.dimp <= 128 ? narrow : wide; };
-    auto fn = g.taps == 0   ? pick(k_kv8_rows<TR, 1, 0>, k_kv8_rows<TR, 2, 0>)
-              : g.taps == 3 ? pick(k_kv8_rows<TR, 1, 3>, k_kv8_rows<TR, 2, 3>)
-                            : pick(k_kv8_rows<TR, 1, -1>, k_kv8_rows<TR, 2, -1>);
-    hipLaunchKernelGGL(fn, grid, dim3(256), 0, s, c, (const TR *)rows, ld, pos, n, (TR *)q, ldq);
+    const int chunks = std::min(heads, std::max({1, (heads + 7) / 8, 1280 / blocks}));  // (of heads: all of them where the tokens alone fill the chip, up to eight by a wave in turn)
+    const int values = g.queries_only ? 0 : ((n + 62) / 32 + 3) / 4 * (int)g.kv_heads;
+    hipLaunchKernelGGL((few ? k_kv8_rows<TR, KL, VL, TAPS, 1> : k_kv8_rows<TR, KL, VL, TAPS, 4>), dim3((size_t)blocks * chunks + values), dim3(256), 0, s, c, (const TR *)rows, ld, pos, n, (TR *)q, ldq, blocks, chunks);
     return hipGetLastError();
 }
+template <class TR, int TAPS>
+static hipError_t rows_go(const Kv8 &c, const void *rows, size_t ld, const int *pos, int n, void *q, size_t ldq, hipStream_t s) {
+    if (c.g.dimp > 128 || c.g.vdimp > 128) return rows_launch<TR, 32, 32, TAPS>(c, rows, ld, pos, n, q, ldq, s);
+    if (c.g.dimp > 64) return rows_launch<TR, 16, 16, TAPS>(c, rows, ld, pos, n, q, ldq, s);
+    return c.g.vdimp > 64 ? rows_launch<TR, 8, 16, TAPS>(c, rows, ld, pos, n, q, ldq, s) : rows_launch<TR, 8, 8, TAPS>(c, rows, ld, pos, n, q, ldq, s);
+}
+template <class TR>
+static hipError_t rows_taps(const Kv8 &c, const void *rows, size_t ld, const int *pos, int n, void *q, size_t ldq, hipStream_t s) {
+    return c.g.taps == 0 ? rows_go<TR, 0>(c, rows, ld, pos, n, q, ldq, s) : c.g.taps == 3 ? rows_go<TR, 3>(c, rows, ld, pos, n, q, ldq, s) : rows_go<TR, -1>(c, rows, ld, pos, n, q, ldq, s);
+}
 hipError_t launch_kv8_rows(const Kv8 &c, const void *rows, size_t ld, int rows_f32, const int *pos, int n, void *q, size_t ldq, hipStream_t s) {
-    return rows_f32 ? rows_go<float>(c, rows, ld, pos, n, q, ldq, s) : rows_go<uint16_t>(c, rows, ld, pos, n, q, ldq, s);
+    return rows_f32 ? rows_taps<float>(c, rows, ld, pos, n, q, ldq, s) : rows_taps<uint16_t>(c, rows, ld, pos, n, q, ldq, s);
 }
 
 // ---- positions read back ----------------------------------------------------------------------------------------------

@@ -31,6 +31,8 @@ def test_refusals(built):
         (lambda: hip.kv8_rows_dev(g, 0, 16, 16, 256, True, 8, 1), "16 bytes"),
         (lambda: hip.kv8_rows_dev(g, 16, 16, 16, 255, True, 8, 1), "kv8_rows: bad arguments"),
         (lambda: hip.kv8_rows_dev(g, 16, 16, 16, 256, True, 8, 0), "kv8_rows: bad arguments"),
+        (lambda: hip.kv8_rows_dev(g, 16, 16, 16, 260, True, 8, 2), "kv8_rows: bad arguments"),
+        (lambda: hip.kv8_rows_dev(g, 16, 16, 24, 256, True, 8, 2), "kv8_rows: bad arguments"),
         (lambda: hip.kv8_rows_dev(g, 16, 16, 16, 256, True, 8, 129), "kv8_rows: bad arguments"),
         (lambda: hip.kv8_rows_dev(g, 16, 16, 16, 256, True, 0, 1), "kv8_rows: bad arguments"),
         (lambda: hip.kv8_rows_dev(g, 16, 16, 16, 256, True, 8, 1, 32, 127), "place of the queries"),

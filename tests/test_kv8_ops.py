@@ -67,13 +67,13 @@ def test_written_behind_norms_and_convolutions(hip, pkg, shape, options, f32):
         assert (np.abs(got * scales[..., None] - x) <= scales[..., None] * 0.5 + 1e-5 * largest[..., None]).all()
 
 
-def test_queries_in_place_and_rows_of_odd_leading_dimension(hip, pkg):
+def test_queries_in_place_and_rows_further_apart(hip, pkg):
     t = kv.Attention(pkg, 40, 5, 1, 40, 16)
-    rows = np.full((40, t.ld + 3), 7, np.float32)
+    rows = np.full((40, t.ld + 8), 7, np.float32)
     rows[:, :t.ld] = t.rows
     d = u.dev_bf16(rows)
     pos = u.dev(np.array([0], np.int32))
-    hip.kv8_rows_dev(t.attn, t.cache.ks, t.cache.vs, d, t.ld + 3, False, pos, 40)
+    hip.kv8_rows_dev(t.attn, t.cache.ks, t.cache.vs, d, t.ld + 8, False, pos, 40)
     got, nq = u.host(d), t.heads * t.dimp
     assert np.array_equal(got[:, nq:], rows[:, nq:]) and u.rms_error(got[:, :nq].reshape(40, 5, -1)[..., :40], t.q) < 2.0 ** -8
     before = t.cache.host()

@@ -408,43 +408,90 @@ struct Kv8StepK {
 };
 constexpr float kStepDigits = 8355000.0f;  // below 127 (2^16 + 2^8 + 1): three balanced digits
 
+// a load that leaves no copy in the caches on its way, where kPast holds: a cache read once.  131072 keys of one map: 53.4 -> 48.0 us; in the forms that keep one block (two maps,
+// heads above 128) 8.0 -> 8.4 and 10.5 -> 11.5
+template <bool kPast, class T>
+__device__ __forceinline__ T once(const T *p) {
+    return kPast ? __builtin_nontemporal_load(p) : *p;
+}
+constexpr int step_held(int nk, int nv, int maps) { return nv > 8 || nk * maps >= 4 ? 1 : 2; }  // workgroups a compute unit has registers for
+
 template <int NK, int NV, int MAPS>
-__global__ __launch_bounds__(256, NV > 8 || NK * MAPS >= 4 ? 1 : 2) void k_kv8_step(Kv8StepK p) {
+__global__ __launch_bounds__(256, step_held(NK, NV, MAPS)) void k_kv8_step(Kv8StepK p) {
     extern __shared__ __attribute__((aligned(16))) uint8_t area[];  // digits of the queries [maps][3][16][QS]; then the waves' outputs
     __shared__ float sm[4][MAPS][16], sl[4][MAPS][16], qscale[MAPS][16], news[MAPS + 1];
     __shared__ __attribute__((aligned(16))) int8_t newk[MAPS][NK * 64], newv[NV * 16];
-    constexpr int QS = NK * 64 + 32, J = NK, JV = (NV * 16 + 63) / 64;
+    constexpr int QS = NK * 64 + 32, J = NK, JV = (NV * 16 + 63) / 64, QR = NK > 2 ? 1 : 4;  // QR: rows of a wave at a time
+    // (every argument at once: read where they are used they are a chain of scalar loads)
+    asm volatile("" ::"s"(p.row), "s"(p.q_weight), "s"(p.k_weight), "s"(p.q_factor), "s"(p.rope_cos), "s"(p.rope_sin), "s"(p.far_weight), "s"(p.far_rate), "s"(p.pos), "s"(p.K), "s"(p.V),
+                 "s"(p.k_scale), "s"(p.v_scale), "s"(p.scratch), "s"(p.eps), "s"(p.heads), "s"(p.group), "s"(p.dim), "s"(p.dimp), "s"(p.vdimp), "s"(p.capacity), "s"(p.turned), "s"(p.chunk),
+                 "s"(p.window), "s"(p.normed), "s"(p.append), "s"(p.k_at), "s"(p.v_at));
+    const int posv = *p.pos;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r16 = lane & 15, g = lane >> 4;
-    const int kv = blockIdx.x, first_head = blockIdx.y * 16, h0 = kv * p.group + first_head, nh = min(16, p.group - first_head);
-    const int dimp = p.dimp, vdimp = p.vdimp, pos = __builtin_amdgcn_readfirstlane(*p.pos), n_keys = pos + 1;
+    const int kv = blockIdx.x, first_head = blockIdx.y * 16, h0 = kv * p.group + first_head, nh = min(16, p.group - first_head), dimp = p.dimp, vdimp = p.vdimp;
+    // What does not hang on the position: rows of queries (head, map), a wave every fourth; the new key of map 3 - wave; the new value, wave 0.
+    float x[QR][J], wq[J], wk[J], own[J > JV ? J : JV];
+    auto row_of = [&](int i0) {
+#pragma unroll
+        for (int i = 0; i < QR; ++i) {
+            const float *src = p.row + (size_t)(h0 * MAPS + min(wave + 4 * (i0 + i), nh * MAPS - 1)) * dimp;
+#pragma unroll
+            for (int j = 0; j < J; ++j) x[i][j] = lane + 64 * j < dimp ? src[lane + 64 * j] : 0.f;
+        }
+    };
+    row_of(0);
+    const bool writes_key = p.append && 3 - wave < MAPS, writes_value = p.append && wave == 0;
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+        const int at = min(lane + 64 * j, p.dim - 1);
+        wq[j] = wk[j] = 1.0f;
+        if (p.q_weight) wq[j] = p.q_weight[at];
+        if (p.k_weight) wk[j] = p.k_weight[at];
+    }
+    if (writes_value) {
+#pragma unroll
+        for (int j = 0; j < JV; ++j) own[j] = lane + 64 * j < vdimp ? p.row[p.v_at + kv * vdimp + lane + 64 * j] : 0.f;
+    } else if (writes_key) {
+#pragma unroll
+        for (int j = 0; j < J; ++j) own[j] = lane + 64 * j < dimp ? p.row[p.k_at + (kv * MAPS + 3 - wave) * dimp + lane + 64 * j] : 0.f;
+    }
+    const int pos = __builtin_amdgcn_readfirstlane(posv), n_keys = pos + 1;
     int first = p.chunk ? pos - (int)((unsigned)pos % (unsigned)p.chunk) : 0;  // gqa_range
     if (p.window && pos - p.window + 1 > first) first = pos - p.window + 1;
-    const int base = first & ~(kGqaTile - 1), tiles = (n_keys - base + kGqaTile - 1) / kGqaTile, per = (tiles + kGqaSplits - 1) / kGqaSplits, used = (tiles + per - 1) / per;
-    if ((int)blockIdx.z >= used) return;
-    const int k0 = base + blockIdx.z * per * kGqaTile, k1 = min(k0 + per * kGqaTile, n_keys);
+    const int base = first & ~(kGqaTile - 1), tiles = (n_keys - base + kGqaTile - 1) / kGqaTile, per = (tiles + kGqaSplits - 1) / kGqaSplits, used = per == 1 ? tiles : (tiles + per - 1) / per;
+    // More workgroups than the chip holds at once would each pay for the queries again: neighbouring records become one, and those behind it empty.
+    constexpr int kHeld = 256 * step_held(NK, NV, MAPS);
+    const int wide = (int)(gridDim.x * gridDim.y) * used, take = wide > 2 * kHeld ? 4 : wide > kHeld ? 2 : 1, record = blockIdx.z * take;
+    if (record >= used) return;
+    const int k0 = base + record * per * kGqaTile, k1 = min(k0 + take * per * kGqaTile, n_keys);
     int8_t *K = p.K + (size_t)kv * MAPS * p.capacity * dimp, *V = p.V + (size_t)kv * vdimp * p.capacity;
     float *KS = p.k_scale + (size_t)kv * MAPS * p.capacity, *VS = p.v_scale + (size_t)kv * p.capacity;
-    i32x4 kf[2][MAPS][NK];
-    u32x4 vf[NV / 2];
-    f32x4 sk[MAPS][2], sv[2];
-    auto fetch_keys = [&](int kb) {  // (blocks lie below the capacity, a multiple of 128)
+    // the next block on its way while this one is worked on, where registers allow it; else from the last use of the registers on
+    constexpr bool kTwo = NK <= 2 && NV * MAPS <= 8;
+    struct Block {
+        i32x4 k[2][MAPS][NK];
+        u32x4 v[NV / 2];
+        f32x4 sk[MAPS][2], sv[2];
+    };
+    auto fetch_keys = [&](Block &b, int kb) {  // (blocks lie below the capacity, a multiple of 128)
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int j = 0; j < MAPS; ++j) {
 #pragma unroll
                 for (int kk = 0; kk < NK; ++kk)
-                    kf[t][j][kk] = *reinterpret_cast<const i32x4 *>(K + ((size_t)j * p.capacity + kb + (r16 >> 2) * 8 + t * 4 + (r16 & 3)) * dimp + min(kk * 64 + g * 16, dimp - 16));
-                sk[j][t] = *reinterpret_cast<const f32x4 *>(KS + (size_t)j * p.capacity + kb + g * 8 + t * 4);
+                    b.k[t][j][kk] = once<kTwo>(reinterpret_cast<const i32x4 *>(K + ((size_t)j * p.capacity + kb + (r16 >> 2) * 8 + t * 4 + (r16 & 3)) * dimp + min(kk * 64 + g * 16, dimp - 16)));
+                b.sk[j][t] = *reinterpret_cast<const f32x4 *>(KS + (size_t)j * p.capacity + kb + g * 8 + t * 4);
             }
     };
-    auto fetch_values = [&](int kb) {
+    auto fetch_values = [&](Block &b, int kb) {
 #pragma unroll
-        for (int v = 0; v < NV / 2; ++v) vf[v] = *reinterpret_cast<const u32x4 *>(V + (size_t)kb * vdimp + min(v, (vdimp >> 5) - 1) * 1024 + r16 * 64 + g * 16);
+        for (int v = 0; v < NV / 2; ++v) b.v[v] = once<kTwo>(reinterpret_cast<const u32x4 *>(V + (size_t)kb * vdimp + min(v, (vdimp >> 5) - 1) * 1024 + r16 * 64 + g * 16));
 #pragma unroll
-        for (int t = 0; t < 2; ++t) sv[t] = *reinterpret_cast<const f32x4 *>(VS + kb + g * 8 + t * 4);
+        for (int t = 0; t < 2; ++t) b.sv[t] = *reinterpret_cast<const f32x4 *>(VS + kb + g * 8 + t * 4);
     };
-    if (k0 + wave * 32 < k1) fetch_keys(k0 + wave * 32), fetch_values(k0 + wave * 32);
+    Block blocks[kTwo ? 2 : 1];
+    if (k0 + wave * 32 < k1) fetch_keys(blocks[0], k0 + wave * 32), fetch_values(blocks[0], k0 + wave * 32);
     float cs[J], sn[J];
 #pragma unroll
     for (int j = 0; j < J; ++j) {
@@ -454,19 +501,17 @@ __global__ __launch_bounds__(256, NV > 8 || NK * MAPS >= 4 ? 1 : 2) void k_kv8_s
             cs[j] = p.rope_cos[at], sn[j] = p.rope_sin[at];
         }
     }
+    const float factor = p.q_factor[pos];
     // a row of a head, elements lane + 64 j: norm, weight, rotation by pairs of neighbours; the largest of them, INFINITY if one is not finite
-    auto finished = [&](const float *src, const float *weight, bool normed, float factor, float (&x)[J]) {
+    auto finished = [&](float (&x)[J], const float (&weight)[J], bool normed, float factor) {
         float ss = 0.f, largest = 0.f;
 #pragma unroll
-        for (int j = 0; j < J; ++j) {
-            x[j] = lane + 64 * j < dimp ? src[lane + 64 * j] : 0.f;
-            ss += x[j] * x[j];
-        }
+        for (int j = 0; j < J; ++j) ss += x[j] * x[j];
         if (normed) factor *= 1.0f / sqrtf(wave_sum(ss) / (float)p.dim + p.eps);
 #pragma unroll
         for (int j = 0; j < J; ++j) {
             const int i = lane + 64 * j;
-            x[j] *= factor * (weight && i < p.dim ? weight[i] : 1.0f);
+            x[j] *= factor * (i < p.dim ? weight[j] : 1.0f);
             if (p.turned) {
                 const float o = dpp<0xb1>(x[j]);  // quad_perm [1,0,3,2]
                 if (i < p.turned) x[j] = (i & 1) ? x[j] * cs[j] + o * sn[j] : x[j] * cs[j] - o * sn[j];
@@ -476,54 +521,57 @@ __global__ __launch_bounds__(256, NV > 8 || NK * MAPS >= 4 ? 1 : 2) void k_kv8_s
         return rows_max(row_max(largest));
     };
     const bool owner = k1 == n_keys && p.append;
-    if (owner && 3 - wave < MAPS) {  // the record that holds the new position appends it (and puts it into its own fragments below)
-        const int j = 3 - wave;
-        float x[J];
-        const float largest = finished(p.row + p.k_at + (kv * MAPS + j) * dimp, p.k_weight, p.normed & 2, 1.0f, x);
-        const Kv8Scale s = kv8_scale(largest, is_finite(largest));
+    if (owner && writes_value) {
+        float largest = 0.f;
 #pragma unroll
-        for (int i = 0; i < J; ++i)
-            if (lane + 64 * i < dimp) {
-                const int8_t b = (int8_t)kv8_number(x[i], s);
-                K[((size_t)j * p.capacity + pos) * dimp + lane + 64 * i] = b;
-                newk[j][lane + 64 * i] = b;
-            }
-        if (lane == 0) KS[(size_t)j * p.capacity + pos] = s.scale, news[j] = s.scale;
-    }
-    if (owner && wave == 0) {
-        float x[JV], largest = 0.f;
-#pragma unroll
-        for (int i = 0; i < JV; ++i) {
-            x[i] = lane + 64 * i < vdimp ? p.row[p.v_at + kv * vdimp + lane + 64 * i] : 0.f;
-            largest = fmaxf(largest, is_finite(x[i]) ? fabsf(x[i]) : INFINITY);
-        }
+        for (int i = 0; i < JV; ++i) largest = fmaxf(largest, is_finite(own[i]) ? fabsf(own[i]) : INFINITY);
         largest = rows_max(row_max(largest));
         const Kv8Scale s = kv8_scale(largest, is_finite(largest));
 #pragma unroll
         for (int i = 0; i < JV; ++i)
             if (lane + 64 * i < vdimp) {
-                const int8_t b = (int8_t)kv8_number(x[i], s);
+                const int8_t b = (int8_t)kv8_number(own[i], s);
                 V[kv8_value_at(vdimp, pos, lane + 64 * i)] = b;
                 newv[lane + 64 * i] = b;
             }
         if (lane == 0) VS[pos] = s.scale, news[MAPS] = s.scale;
-    }
-    const float factor = p.q_factor[pos];
-    for (int r = wave; r < nh * MAPS; r += 4) {  // (head, map)
-        const int hh = r / MAPS, j = r - hh * MAPS;
-        float x[J];
-        const float largest = finished(p.row + ((size_t)(h0 + hh) * MAPS + j) * dimp, p.q_weight, p.normed & 1, factor, x);
-        const bool live = largest >= 1e-30f && is_finite(largest);
-        const float to = live ? kStepDigits / largest : 0.f;
-        uint8_t *dst = area + (size_t)(j * 3 * 16 + hh) * QS;
+    } else if (owner && writes_key) {  // the record that holds the new position appends it (and puts it into its own fragments below)
+        const int j = 3 - wave;
+        float key[J];
 #pragma unroll
-        for (int i = 0; i < J; ++i) {
-            const int v = live ? (int)rintf(x[i] * to) : 0, d0 = (int)(int8_t)v, v1 = (v - d0) >> 8, d1 = (int)(int8_t)v1, d2 = (v1 - d1) >> 8;
-            dst[lane + 64 * i] = (uint8_t)d0, dst[16 * QS + lane + 64 * i] = (uint8_t)d1, dst[32 * QS + lane + 64 * i] = (uint8_t)d2;
+        for (int i = 0; i < J; ++i) key[i] = own[i];
+        const float largest = finished(key, wk, p.normed & 2, 1.0f);
+        const Kv8Scale s = kv8_scale(largest, is_finite(largest));
+#pragma unroll
+        for (int i = 0; i < J; ++i)
+            if (lane + 64 * i < dimp) {
+                const int8_t b = (int8_t)kv8_number(key[i], s);
+                K[((size_t)j * p.capacity + pos) * dimp + lane + 64 * i] = b;
+                newk[j][lane + 64 * i] = b;
+            }
+        if (lane == 0) KS[(size_t)j * p.capacity + pos] = s.scale, news[j] = s.scale;
+    }
+    for (int i0 = 0; wave + 4 * i0 < nh * MAPS; i0 += QR) {
+        if (i0) row_of(i0);
+#pragma unroll
+        for (int i = 0; i < QR; ++i) {
+            const int at = wave + 4 * (i0 + i), hh = at / MAPS, j = at - hh * MAPS;  // (head, map)
+            if (at >= nh * MAPS) continue;
+            const float largest = finished(x[i], wq, p.normed & 1, factor);
+            const bool live = largest >= 1e-30f && is_finite(largest);
+            const float to = live ? kStepDigits / largest : 0.f;
+            uint8_t *dst = area + (size_t)(j * 3 * 16 + hh) * QS;
+#pragma unroll
+            for (int e = 0; e < J; ++e) {
+                const int v = live ? (int)rintf(x[i][e] * to) : 0, d0 = (int)(int8_t)v, v1 = (v - d0) >> 8, d1 = (int)(int8_t)v1, d2 = (v1 - d1) >> 8;
+                dst[lane + 64 * e] = (uint8_t)d0, dst[16 * QS + lane + 64 * e] = (uint8_t)d1, dst[32 * QS + lane + 64 * e] = (uint8_t)d2;
+            }
+            if (lane == 0) qscale[j][hh] = is_finite(largest) ? largest * (kLog2e / kStepDigits) : __builtin_nanf("");
         }
-        if (lane == 0) qscale[j][hh] = is_finite(largest) ? largest / kStepDigits : __builtin_nanf("");
     }
     __syncthreads();
+    constexpr bool kInLds = NK * MAPS > 4;  // (two maps of the largest heads: their queries stay there)
+    auto digits = [&](int j, int d, int kk) { return *reinterpret_cast<const i32x4 *>(area + (size_t)((j * 3 + d) * 16 + r16) * QS + kk * 64 + g * 16); };
     i32x4 q[MAPS][3][NK];  // (lanes past the last head: whatever lies there; a column of the products is a head of its own)
     float qs[MAPS];
 #pragma unroll
@@ -532,10 +580,10 @@ __global__ __launch_bounds__(256, NV > 8 || NK * MAPS >= 4 ? 1 : 2) void k_kv8_s
 #pragma unroll
         for (int d = 0; d < 3; ++d)
 #pragma unroll
-            for (int kk = 0; kk < NK; ++kk) q[j][d][kk] = *reinterpret_cast<const i32x4 *>(area + (size_t)((j * 3 + d) * 16 + r16) * QS + kk * 64 + g * 16);
+            for (int kk = 0; kk < NK; ++kk) q[j][d][kk] = kInLds ? i32x4{0, 0, 0, 0} : digits(j, d, kk);
     }
     FarPenalty far{0.f, 0.f};
-    if (p.far_weight) far.weight = p.far_weight[min(h0 + r16, p.heads - 1)] * 0.69314718055994531f, far.rate = p.far_rate[min(h0 + r16, p.heads - 1)];
+    if (p.far_weight) far.weight = p.far_weight[min(h0 + r16, p.heads - 1)], far.rate = p.far_rate[min(h0 + r16, p.heads - 1)];
     f32x4 o[NV][MAPS];
     float m[MAPS], l[MAPS];
 #pragma unroll
@@ -545,12 +593,17 @@ __global__ __launch_bounds__(256, NV > 8 || NK * MAPS >= 4 ? 1 : 2) void k_kv8_s
         for (int v = 0; v < NV; ++v) o[v][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
     int above = -100;
-    for (int kb = k0 + wave * 32; kb < k1; kb += 128) {
+    auto work = [&](int kb, Block &now, Block &then) __attribute__((always_inline)) {
         const bool more = kb + 128 < k1;
+        if (kTwo && more) fetch_keys(then, kb + 128), fetch_values(then, kb + 128);
         if (kb + 32 <= first) {  // (another chunk's keys)
-            if (more) fetch_keys(kb + 128), fetch_values(kb + 128);
-            continue;
+            if (!kTwo && more) fetch_keys(then, kb + 128), fetch_values(then, kb + 128);
+            return;
         }
+        auto &kf = now.k;
+        auto &vf = now.v;
+        auto &sk = now.sk;
+        auto &sv = now.sv;
         if (owner && pos - kb < 32) {  // the new position, which memory need not show yet
             const int at = pos - kb, t = (at >> 2) & 1;
             const bool mine = r16 == (at >> 3) * 4 + (at & 3);
@@ -582,17 +635,14 @@ __global__ __launch_bounds__(256, NV > 8 || NK * MAPS >= 4 ? 1 : 2) void k_kv8_s
                     }
             }
         }
-        float largest = 0.f;
-        bool seen[2][4];
+        const bool whole = kb >= first && kb + 32 <= k1;
+        auto seen = [&](int t, int e) { return kb + g * 8 + t * 4 + e < k1 && kb + g * 8 + t * 4 + e >= first; };
+        if (!whole)
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+            for (int t = 0; t < 2; ++t)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int key = kb + g * 8 + t * 4 + e;
-                seen[t][e] = key < k1 && key >= first;
-                sv[t][e] = seen[t][e] ? sv[t][e] : 0.f;
-                largest = fmaxf(largest, sv[t][e]);
-            }
+                for (int e = 0; e < 4; ++e) sv[t][e] = seen(t, e) ? sv[t][e] : 0.f;
+        const float largest = fmaxf(fmaxf(fmaxf(sv[0][0], sv[0][1]), fmaxf(sv[0][2], sv[0][3])), fmaxf(fmaxf(sv[1][0], sv[1][1]), fmaxf(sv[1][2], sv[1][3])));
         const int need = __builtin_amdgcn_readfirstlane(exponent_above(rows_max(largest)));
         if (need > above) {
             const float down = power2(max(above - need, -140));
@@ -613,26 +663,35 @@ __global__ __launch_bounds__(256, NV > 8 || NK * MAPS >= 4 ? 1 : 2) void k_kv8_s
                 for (int d = 0; d < 3; ++d) {
                     a[d] = i32x4{0, 0, 0, 0};
 #pragma unroll
-                    for (int kk = 0; kk < NK; ++kk) a[d] = mfma_i8(kf[t][j][kk], q[j][d][kk], a[d]);  // (columns past dimp: the query is zero there)
+                    for (int kk = 0; kk < NK; ++kk) a[d] = mfma_i8(kf[t][j][kk], kInLds ? digits(j, d, kk) : q[j][d][kk], a[d]);  // (columns past dimp: the query is zero there)
                 }
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    s[t][e] = fmaf((float)a[2][e], 65536.0f, fmaf((float)a[1][e], 256.0f, (float)a[0][e])) * (sk[j][t][e] * qs[j]);
+                    s[t][e] = fmaf((float)a[2][e], 65536.0f, fmaf((float)a[1][e], 256.0f, (float)a[0][e])) * (sk[j][t][e] * qs[j]);  // (qs holds log2(e))
                     if (MAPS == 1 && p.far_weight) s[t][e] = nearer(s[t][e], far, pos - (kb + g * 8 + t * 4 + e));
-                    s[t][e] = seen[t][e] ? s[t][e] * kLog2e : -INFINITY;
                 }
             }
+            if (!whole)
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[t][e] = seen(t, e) ? s[t][e] : -INFINITY;
             float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
             mx = fmaxf(m[j], rows_max(mx));
-            if (mx == -INFINITY) mx = 0.f;  // (no score is a number: neither is the sum)
-            const float al = __builtin_amdgcn_exp2f(m[j] - mx);
-            m[j] = mx;
+            if (__any(mx > m[j] || mx == -INFINITY)) {
+                if (mx == -INFINITY) mx = 0.f;  // (no score is a number: neither is the sum)
+                const float al = __builtin_amdgcn_exp2f(m[j] - mx);
+                m[j] = mx;
+                l[j] *= al;
+#pragma unroll
+                for (int v = 0; v < NV; ++v) o[v][j] *= al;
+            }
             f32x4 w[2];
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) w[t][e] = __builtin_amdgcn_exp2f(s[t][e] - mx);
-            l[j] = l[j] * al + ((w[0][0] + w[0][1]) + (w[0][2] + w[0][3])) + ((w[1][0] + w[1][1]) + (w[1][2] + w[1][3]));
+            l[j] += ((w[0][0] + w[0][1]) + (w[0][2] + w[0][3])) + ((w[1][0] + w[1][1]) + (w[1][2] + w[1][3]));
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -643,10 +702,8 @@ __global__ __launch_bounds__(256, NV > 8 || NK * MAPS >= 4 ? 1 : 2) void k_kv8_s
                     hi[j][4 * t + e] = h.x, hi[j][4 * t + e + 1] = h.y;
                     lo[j][4 * t + e] = (_Float16)(x - (float)h.x), lo[j][4 * t + e + 1] = (_Float16)(y - (float)h.y);
                 }
-#pragma unroll
-            for (int v = 0; v < NV; ++v) o[v][j] *= al;
         }
-        if (more) fetch_keys(kb + 128);
+        if (!kTwo && more) fetch_keys(then, kb + 128);
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
             const f16x8 a = eight_f16(vf[v / 2][2 * (v & 1)], vf[v / 2][2 * (v & 1) + 1]);
@@ -656,7 +713,11 @@ __global__ __launch_bounds__(256, NV > 8 || NK * MAPS >= 4 ? 1 : 2) void k_kv8_s
                 o[v][j] = mfma_f16(a, lo[j], o[v][j]);
             }
         }
-        if (more) fetch_values(kb + 128);
+        if (!kTwo && more) fetch_values(then, kb + 128);
+    };
+    for (int kb = k0 + wave * 32; kb < k1; kb += kTwo ? 256 : 128) {
+        work(kb, blocks[0], blocks[kTwo ? 1 : 0]);
+        if (kTwo && kb + 128 < k1) work(kb + 128, blocks[kTwo ? 1 : 0], blocks[0]);
     }
 #pragma unroll
     for (int j = 0; j < MAPS; ++j) {
@@ -683,7 +744,12 @@ __global__ __launch_bounds__(256, NV > 8 || NK * MAPS >= 4 ? 1 : 2) void k_kv8_s
     const int n_rows = MAPS * nh;
     for (int r = tid >> 5; r < n_rows; r += 8) {
         const int j = MAPS == 2 && r >= nh ? 1 : 0, hh = r - j * nh;
-        float *rec = p.scratch + ((size_t)((h0 + hh) * MAPS + j) * kGqaSplits + blockIdx.z) * (kGqaRecHead + vdimp);
+        float *rec = p.scratch + ((size_t)((h0 + hh) * MAPS + j) * kGqaSplits + record) * (kGqaRecHead + vdimp);
+        for (int e = 1; e < min(take, used - record); ++e) {
+            float *empty = rec + (size_t)e * (kGqaRecHead + vdimp);
+            for (int c = (tid & 31) * 4; c < vdimp; c += 128) *reinterpret_cast<f32x4 *>(empty + kGqaRecHead + c) = f32x4{0.f, 0.f, 0.f, 0.f};
+            if ((tid & 31) == 0) empty[0] = -INFINITY, empty[1] = 0.f;
+        }
         for (int c = (tid & 31) * 4; c < vdimp; c += 128) {
             const float *src = outs + (size_t)r * vdimp + c;
             const size_t step = (size_t)n_rows * vdimp;

@@ -200,6 +200,16 @@ def test_step_behind_many_keys(hip, pkg, n, window):
     t.check(t.step(hip, n - 1), t.want(t.q[n - 1:], n - 1), STEP * 3)
 
 
+@pytest.mark.parametrize("shape,n", [((20, 20, 32, 32, 1), 8000), ((10, 5, 64, 64, 1), 16200), ((3, 3, 200, 200, 1), 12800), ((12, 12, 32, 64, 2), 5700), ((40, 40, 64, 64, 1), 13 * 128 + 1)])
+def test_step_of_more_records_than_the_chip_holds_at_once(hip, pkg, shape, n):
+    """neighbouring records become one; what lay in their places is gone"""
+    t = kv.Attention(pkg, n, *shape)
+    t.fill(hip, 0, n - 1)
+    scratch = u.zeros_f32(hip.gqa_scratch_bytes(t.heads, t.maps, t.vdimp, 1) // 4)
+    scratch.fill_(np.nan)
+    t.check(t.step(hip, n - 1, scratch=scratch), t.want(t.q[n - 1:], n - 1), STEP * 3)
+
+
 @pytest.mark.parametrize("spread", [1e-30, 1e-3, 1e3, 1e30])
 def test_values_of_very_different_size(hip, pkg, spread):
     """scales grow and shrink by the token: what is large decides, whatever came ahead of it"""

@@ -860,11 +860,10 @@ __global__ __launch_bounds__(64 * W * G, NV > 8 || NK > 2 ? 1 : 2) void k_kv8_pr
             }
         raised[t] = -1152.0f * rows_sum(total);
         // (finite: with chunks a tile may hold no key that a query sees)
-        const bool sink = MAPS == 1 && p.sink && grp == 0 && !records;
-        m[t] = sink ? p.sink[h] * kLog2e : -1e30f;
+        m[t] = -1e30f;
         if (FAR && MAPS == 1) far[t] = far_penalty(p, h), far[t].weight *= kLog2e;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) l[t][i] = sink ? power2((int)kWeightUp) : 0.f;
+        for (int i = 0; i < 4; ++i) l[t][i] = 0.f;
 #pragma unroll
         for (int v = 0; v < NV; ++v) o[v][t] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
@@ -1148,7 +1147,13 @@ __global__ __launch_bounds__(64 * W * G, NV > 8 || NK > 2 ? 1 : 2) void k_kv8_pr
     }
     float inv[SLOTS];
 #pragma unroll
-    for (int t = 0; t < SLOTS; ++t) inv[t] = 1.0f / sum[t];
+    for (int t = 0; t < SLOTS; ++t) {
+        inv[t] = 1.0f / sum[t];
+        if (MAPS == 1 && p.sink) {  // (behind the keys: as their first maximum one far above them would leave their weights no bits)
+            const float z = p.sink[head[t / MAPS]] * kLog2e, M = fmaxf(m[t], z), w = __builtin_amdgcn_exp2f(m[t] - M);
+            inv[t] = w / (sum[t] * w + __builtin_amdgcn_exp2f(z - M));
+        }
+    }
     if (MAPS == 2) {
         float ss = 0.f;
 #pragma unroll

@@ -311,6 +311,21 @@ def test_queries_without_numbers(hip, pkg):
     assert u.rms_error(got[60, 0], mean) < sum(PROMPT)
 
 
+@pytest.mark.parametrize("sink", [-60.0, 12.0, 20.0, 60.0])
+def test_sinks_far_from_every_score(hip, pkg, sink):
+    """one far above leaves small outputs, to as many bits as others"""
+    n = 300
+    t = kv.Attention(pkg, n, 6, 2, 64, 64, sink=True)
+    t.sink[:] = sink + np.arange(6)
+    t.keep.append(u.dev_f32(t.sink))
+    t.attn.sink = t.keep[-1].data_ptr()
+    _, q = t.fill(hip, 0, n)
+    want = t.want(u.host(q).reshape(n, -1, t.dimp)[..., :t.dim], 0)
+    for split in (True, False):
+        t.check(t.prompt(hip, q, 0, n, split), want, *PROMPT)
+    t.check(t.step(hip, n - 1), t.want(t.q[n - 1:], n - 1), STEP)
+
+
 # ---- together -----------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("shape", [(20, 5, 128, 128, 1), (12, 3, 64, 128, 2), (6, 2, 96, 96, 1)])
 def test_a_sequence_as_it_is_used(hip, pkg, shape):

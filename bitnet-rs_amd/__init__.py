@@ -212,6 +212,14 @@ class HipLib:
         L.bitnet_hip_gemv_fused_dev.argtypes = [C.c_uint64, _vp, _vp, _sz, _vp, C.c_float, _vp, C.c_int, _vp]
         L.bitnet_hip_rmsnorm.argtypes = [_f32p, _sz, _f32p, _sz, _f32p, _sz, _sz, _sz, C.c_float]
         L.bitnet_hip_norm_rows_dev.argtypes = [_vp, _vp, _vp, _sz, _sz, C.c_float, C.c_int, _vp]
+        gqa = C.POINTER(Gqa)
+        L.bitnet_hip_gqa_merge_dev.argtypes = [gqa, _vp, _sz, _sz, _vp, _vp, _sz, C.c_int, _vp]
+        L.bitnet_hip_kv8_rows_dev.argtypes = [gqa, _vp, _vp, _vp, _sz, C.c_int, _vp, _sz, _vp, _sz, _vp]
+        L.bitnet_hip_kv8_read_dev.argtypes = [gqa, _vp, _vp, _sz, _sz, _vp, _vp, C.c_int, _vp]
+        L.bitnet_hip_kv8_step_dev.argtypes = [gqa, _vp, _vp, _vp, _vp, _vp, _vp]
+        L.bitnet_hip_kv8_prefill_scratch_bytes.argtypes = [gqa, _sz, _sz]
+        L.bitnet_hip_kv8_prefill_scratch_bytes.restype = _sz
+        L.bitnet_hip_kv8_prefill_dev.argtypes = [gqa, _vp, _vp, _vp, _sz, _sz, _sz, _vp, _sz, _vp, _sz, _vp]
         L.bitnet_hip_embed_f16_dev.argtypes = [_vp, _vp, _vp, _sz, _sz, _sz, _vp, _vp]
         L.bitnet_hip_advance_pos_dev.argtypes = [_vp, _vp]
         L.bitnet_hip_attention_decode_dev.argtypes = [_vp, _vp, _vp, _vp, _vp, _sz, _sz, _sz, _sz, _vp, _vp, _vp, _vp]
@@ -653,7 +661,7 @@ class HipLib:
         self._call("gqa_project_dev", C.byref(a), _ptr(pos), _sz(records), _ptr(scratch), _ptr(w), _sz(rows), _sz(cols), _sz(ld), _optr(bias), _ptr(y), _vp(stream))
 
     def gqa_merge_dev(self, a: "Gqa", pos, q0: int, nq: int, scratch, out, ldo: int, out_bf16: bool, stream: int = 0) -> None:
-        self._call("gqa_merge_dev", C.byref(a), _ptr(pos), _sz(q0), _sz(nq), _ptr(scratch), _ptr(out), _sz(ldo), C.c_int(out_bf16), _vp(stream))
+        self._check(self.c.bitnet_hip_gqa_merge_dev(C.byref(a), _addr(pos), q0, nq, _addr(scratch), _addr(out), ldo, out_bf16, stream))
 
     def gqa_prefill_dev(self, a: "Gqa", q, ldq: int, n_ctx: int, nq: int, out, ldo: int, stream: int = 0) -> None:
         self._call("gqa_prefill_dev", C.byref(a), _ptr(q), _sz(ldq), _sz(n_ctx), _sz(nq), _ptr(out), _sz(ldo), _vp(stream))
@@ -669,20 +677,19 @@ class HipLib:
         return int(self.c.bitnet_hip_gqa_prefill_last_groups())
 
     def kv8_rows_dev(self, a: "Gqa", k_scale, v_scale, rows, ld: int, rows_f32: bool, pos, n: int, q=None, ldq: int = 0, stream: int = 0) -> None:
-        self._call("kv8_rows_dev", C.byref(a), _ptr(k_scale), _ptr(v_scale), _ptr(rows), _sz(ld), C.c_int(rows_f32), _ptr(pos), _sz(n), _optr(q), _sz(ldq), _vp(stream))
+        self._check(self.c.bitnet_hip_kv8_rows_dev(C.byref(a), _addr(k_scale), _addr(v_scale), _addr(rows), ld, rows_f32, _addr(pos), n, _addr(q), ldq, stream))
 
     def kv8_read_dev(self, a: "Gqa", k_scale, v_scale, first: int, n: int, keys, values, f32: bool, stream: int = 0) -> None:
-        self._call("kv8_read_dev", C.byref(a), _ptr(k_scale), _ptr(v_scale), _sz(first), _sz(n), _optr(keys), _optr(values), C.c_int(f32), _vp(stream))
+        self._check(self.c.bitnet_hip_kv8_read_dev(C.byref(a), _addr(k_scale), _addr(v_scale), first, n, _addr(keys), _addr(values), f32, stream))
 
     def kv8_step_dev(self, a: "Gqa", k_scale, v_scale, row, pos, scratch, stream: int = 0) -> None:
-        self._call("kv8_step_dev", C.byref(a), _ptr(k_scale), _ptr(v_scale), _ptr(row), _ptr(pos), _ptr(scratch), _vp(stream))
+        self._check(self.c.bitnet_hip_kv8_step_dev(C.byref(a), _addr(k_scale), _addr(v_scale), _addr(row), _addr(pos), _addr(scratch), stream))
 
     def kv8_prefill_scratch_bytes(self, a: "Gqa", n_ctx: int, nq: int) -> int:
-        self.c.bitnet_hip_kv8_prefill_scratch_bytes.restype = _sz
-        return int(self.c.bitnet_hip_kv8_prefill_scratch_bytes(C.byref(a), _sz(n_ctx), _sz(nq)))
+        return self.c.bitnet_hip_kv8_prefill_scratch_bytes(C.byref(a), n_ctx, nq)
 
     def kv8_prefill_dev(self, a: "Gqa", k_scale, v_scale, q, ldq: int, n_ctx: int, nq: int, out, ldo: int, scratch=None, scratch_bytes: int = 0, stream: int = 0) -> None:
-        self._call("kv8_prefill_dev", C.byref(a), _ptr(k_scale), _ptr(v_scale), _ptr(q), _sz(ldq), _sz(n_ctx), _sz(nq), _ptr(out), _sz(ldo), _optr(scratch), _sz(scratch_bytes), _vp(stream))
+        self._check(self.c.bitnet_hip_kv8_prefill_dev(C.byref(a), _addr(k_scale), _addr(v_scale), _addr(q), ldq, n_ctx, nq, _addr(out), ldo, _addr(scratch), scratch_bytes, stream))
 
     def delta_step_dev(self, d: "Delta", row, ba, pos, out, stream: int = 0) -> None:
         self._call("delta_step_dev", C.byref(d), _ptr(row), _ptr(ba), _ptr(pos), _ptr(out), _vp(stream))

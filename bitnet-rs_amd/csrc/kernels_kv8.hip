@@ -1,7 +1,7 @@
 // kernels_kv8.hip -- the attention of kernels_gqa.hip over caches of 8 bits (gfx950).
 //
 // A head's key (of one map) and a head's value at a position are whole numbers -127 .. 127 with one f32 scale each: value = number * scale (kv8_scale).  One scale
-// per position, not per block of them: an append touches nothing that is written, and the cache is a function of the tokens alone, however they came in.
+// per position, not per block of them: an append touches nothing that is written, and the cache is a function of the tokens alone, whatever portions they came in.
 // Keys int8 [kv head][map][capacity][dimp]; values int8 [kv head][capacity / 32][vdimp / 32][16][4][2][8]: column c at position p lies at [p / 32][c / 32][c % 16]
 // [p % 32 / 8][c % 32 / 16][p % 8], so that 32 keys by 32 columns are 1 KiB in the order in which the matrix cores take them, and 32 keys of a head are one piece.
 //   k_kv8_rows     rows of projections: convolution, norms, rotation, then 8 bits
@@ -73,10 +73,11 @@ __device__ __forceinline__ size_t kv8_value_at(int vdimp, int pos, int c) {
 }
 
 // ---- rows of projections ----------------------------------------------------------------------------------------------
-// Bound by memory: 16384 tokens of 20 heads on 5 of 128 columns, bf16, half of them turned, are 232 MB in 50-52 us (4.5 TB/s; a copy reaches 5.3).  By heads first and pairs of columns it
-// was 80, whole rows at a time 64; a wave's heads in turn, with the rotation and the next columns in registers, took the rest.  One token 4.0, 1531 of two maps of 64 / 128 8.7.
+// Bound by memory: 16384 tokens of 20 heads on 5 of 128 columns, bf16, half of them turned, are 232 MB in 52 us (4.5 TB/s; a copy reaches 5.3).  By heads first and pairs of columns it
+// was 80, whole rows at a time 64; a wave's heads in turn, with the rotation and the next columns in registers, took the rest.  One token 4.1, 1531 of two maps of 64 / 128 9.1.
 // A lane holds eight neighbouring columns, KL or VL lanes a head's row: pairs turn within a lane, and a wave takes 64 / KL tokens at a time, R times.  Workgroups: four waves'
-// tokens and a part of the heads (query heads x maps, key heads x maps; one after the other, the next one's columns on their way), then values, a wave a tile of 32 positions, its rows through LDS into the cache's order.
+// tokens and a part of the heads (query heads x maps, key heads x maps; one after the other, the next one's columns on their way), then values, a wave a tile of 32 positions, its rows
+// through LDS into the cache's order.
 
 template <int L>
 __device__ __forceinline__ float lanes_max(float v) {
@@ -338,6 +339,7 @@ hipError_t launch_kv8_rows(const Kv8 &c, const void *rows, size_t ld, int rows_f
 
 // ---- positions read back ----------------------------------------------------------------------------------------------
 // blockIdx.y: key heads x maps (16 bytes a thread), then value heads (a tile of 32 positions a workgroup, turned round in LDS).
+// Bound by memory: 131072 positions of 8 heads of 128 columns as bf16 are 814 MB in 148 us (5.5 TB/s, what a copy reaches); 300 of 3 heads of 80 as f32 3.0.
 template <class TO>
 __device__ __forceinline__ void store_numbers(TO *dst, uint32_t numbers, float scale) {  // four of them
     f32x4 v;
@@ -399,6 +401,10 @@ hipError_t launch_kv8_read(const Kv8 &c, int first, int n, void *keys, void *val
 // the four meet at the end.  S^T = K Q^T on whole numbers: row 4 g + e of score tile t is key 8 g + 4 t + e of the block, so that a lane's weights of both tiles are the eight
 // consecutive keys 8 g .. 8 g + 7 which it needs as an operand of O^T = V^T P^T.
 // A weight times its value's scale is brought to at most 2^14 by a power of two that the wave keeps (o is held times 2^(14 - above)).
+// Bound by memory behind many keys: 131072 of 32 heads on 8 of 128 columns are 277 MB in 47.6 us (5.8 TB/s; reading alone reaches 6.5).  From 63.5 on: neighbouring records joined where a
+// launch has more of them than the chip holds workgroups, which saves a second preparation of the queries, 53.4; loads past the caches 47.6.  By latency behind few: 200 keys of 20 heads on 5
+// 7.0 us, 2090 of 12 on 3 with two maps of 64 / 128 8.0, 4096 in a window of 16 on 2 of 256 10.5.  A launch is a chain of arguments, position, rows, norms, digits, keys, records: every
+// argument is asked for at once and what does not hang on the position ahead of it (7.5, 8.2 and 11.6 without).
 struct Kv8StepK {
     const float *row, *q_weight, *k_weight, *q_factor, *rope_cos, *rope_sin, *far_weight, *far_rate;
     const int *pos;
@@ -811,6 +817,9 @@ constexpr float kWeightUp = 6.0f, kLazy = 8.0f;
 // times 2^(8 - above)): a rounding of 2^-12 like that of the weights.  The sum of the weights is one more row of the products (ones times the same f16 weights).
 // The products of a SIMD's two waves and their vector instructions take about the same time, and as phases of their own they add up: hence the next tile's scores are made among
 // this tile's exponentials, and this tile's outputs among the staging of the tiles to come.
+// Bound by both pipes of a SIMD: 8192 tokens of 20 heads on 5 of 128 columns, 344 GFLOP, take 393 us (0.87 PFLOP/s, a large product of f16 reaches 1.35; over a cache of bf16 k_gqa_prefill
+// takes 522); 509 tokens behind 20011 of 12 heads on 3 with two maps of 64 / 128 139 us (0.68), 130 tokens of 12 heads 12.3.  Phases one behind the other, two groups of four waves: 515,
+// 226, 11.5.
 // Wave 0 makes the values' factors two tiles ahead, wave 1 the keys' scales.  A value without a scale takes its key's away instead, so that only queries that see it lose theirs.
 // LDS of a tile: keys [maps][64][KS], values [columns][VS]; the 32 bytes behind a row of values hold the keys' scales (rows 16 s + 8 map .., s = 0
 // and 1 in turn), the factors (32 ..) and `above` (36).

@@ -74,10 +74,10 @@ __device__ __forceinline__ size_t kv8_value_at(int vdimp, int pos, int c) {
 
 // ---- rows of projections ----------------------------------------------------------------------------------------------
 // Bound by memory: 16384 tokens of 20 heads on 5 of 128 columns, bf16, half of them turned, are 232 MB in 52 us (4.5 TB/s; a copy reaches 5.3).  By heads first and pairs of columns it
-// was 80, whole rows at a time 64; a wave's heads in turn, with the rotation and the next columns in registers, took the rest.  One token 4.1, 1531 of two maps of 64 / 128 9.1.
+// was 80, whole rows at a time 64; a wave's heads in turn, with the rotation and the next columns in registers, took the rest.  One token 3.8, 1531 of two maps of 64 / 128 7.0.
 // A lane holds eight neighbouring columns, KL or VL lanes a head's row: pairs turn within a lane, and a wave takes 64 / KL tokens at a time, R times.  Workgroups: four waves'
-// tokens and a part of the heads (query heads x maps, key heads x maps; one after the other, the next one's columns on their way), then values, a wave a tile of 32 positions, its rows
-// through LDS into the cache's order.
+// tokens and a part of the heads (query heads x maps, key heads x maps; one after the other, the next one's columns on their way), then values, eight or 32
+// positions a wave, through LDS into the cache's order.
 
 template <int L>
 __device__ __forceinline__ float lanes_max(float v) {
@@ -167,10 +167,10 @@ __device__ __forceinline__ Kv8Scale eight_numbers(const Eight &x, bool live, u32
     return s;
 }
 
-template <class TR, int KL, int VL, int TAPS, int R>
+template <class TR, int KL, int VL, int TAPS, int R, int VP>
 __global__ __launch_bounds__(256) void k_kv8_rows(Kv8 c, const TR *rows, size_t ld, const int *pos_ptr, int n, TR *queries, size_t ldq, int blocks, int chunks) {
     constexpr int PITCH = VL * 8 + 4;
-    __shared__ uint32_t turned_round[4][32][PITCH / 4];
+    __shared__ uint32_t turned_round[4][VP][PITCH / 4];
     const Gqa &p = c.g;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), pos0 = *pos_ptr, channels = gqa_channels(p);
     const int nq = (int)(p.heads * p.maps), nk = (int)(p.kv_heads * p.maps), dim = (int)p.dim, dimp = (int)p.dimp, vdimp = (int)p.vdimp, heads = p.queries_only ? nq : nq + nk;
@@ -260,8 +260,8 @@ __global__ __launch_bounds__(256) void k_kv8_rows(Kv8 c, const TR *rows, size_t 
         }
         return;
     }
-    constexpr int AT_ONCE = 64 / VL, ROUNDS = 32 / AT_ONCE;
-    const int at_block = (int)blockIdx.x - blocks * chunks, block = at_block / (int)p.kv_heads, kv = at_block - block * (int)p.kv_heads, tile = ((pos0 >> 5) + block * 4 + wave) * 32, col = lane % VL * 8, column = (p.values_are_keys ? nq : nq + nk) * dimp + kv * vdimp;
+    constexpr int AT_ONCE = 64 / VL, ROUNDS = VP / AT_ONCE;
+    const int at_block = (int)blockIdx.x - blocks * chunks, block = at_block / (int)p.kv_heads, kv = at_block - block * (int)p.kv_heads, tile = (pos0 / VP + block * 4 + wave) * VP, col = lane % VL * 8, column = (p.values_are_keys ? nq : nq + nk) * dimp + kv * vdimp;
     const bool live = col < vdimp;
     const int at = min(col, vdimp - 8);
     if (tile < pos0 + n) {
@@ -280,10 +280,10 @@ __global__ __launch_bounds__(256) void k_kv8_rows(Kv8 c, const TR *rows, size_t 
     }
     __syncthreads();
     if (tile >= pos0 + n) return;
-    uint8_t *dst = (uint8_t *)p.vcache + (size_t)kv * vdimp * p.capacity + (size_t)tile * vdimp;
+    uint8_t *dst = (uint8_t *)p.vcache + (size_t)kv * vdimp * p.capacity + (size_t)(tile >> 5) * (32 * vdimp);
     // four columns and the four 16 further on, eight positions: two blocks of four by four bytes each, turned
-    for (int i = lane; i < vdimp >> 1; i += 64) {
-        const int p8 = (i & 3) * 8, c4 = i >> 2 & 3, c32 = i >> 4, t8 = tile + p8 - pos0;
+    for (int i = lane; i < (vdimp >> 3) * (VP / 8); i += 64) {
+        const int p8 = i % (VP / 8) * 8, c = i / (VP / 8), c4 = c & 3, c32 = c >> 2, t8 = tile + p8 - pos0;
         uint32_t out[4][4];  // [column][16 bytes: eight positions of it, eight of the one 16 further on]
 #pragma unroll
         for (int h = 0; h < 2; ++h)
@@ -297,7 +297,7 @@ __global__ __launch_bounds__(256) void k_kv8_rows(Kv8 c, const TR *rows, size_t 
                 out[0][2 * h + q] = __builtin_amdgcn_perm(l1, l0, 0x05040100u), out[1][2 * h + q] = __builtin_amdgcn_perm(l1, l0, 0x07060302u);
                 out[2][2 * h + q] = __builtin_amdgcn_perm(h1, h0, 0x05040100u), out[3][2 * h + q] = __builtin_amdgcn_perm(h1, h0, 0x07060302u);
             }
-        uint8_t *to = dst + (c32 * 16 + c4 * 4) * 64 + (i & 3) * 16;
+        uint8_t *to = dst + (c32 * 16 + c4 * 4) * 64 + ((tile + p8) >> 3 & 3) * 16;
         if (t8 >= 0 && t8 + 8 <= n) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) *reinterpret_cast<u32x4 *>(to + e * 64) = u32x4{out[e][0], out[e][1], out[e][2], out[e][3]};
@@ -317,10 +317,12 @@ static hipError_t rows_launch(const Kv8 &c, const void *rows, size_t ld, const i
     const int heads = (int)(g.heads * g.maps + (g.queries_only ? 0 : g.kv_heads * g.maps)), at_once = 4 * 64 / KL;
     const bool few = n <= at_once;  // (a wave takes its tokens at once, else four times as many in turn)
     const int each = few ? at_once : 4 * at_once, blocks = (n + each - 1) / each;
-    // (n tokens from anywhere in a tile of 32 on reach into (n + 62) / 32 of them at most)
     const int chunks = std::min(heads, std::max({1, (heads + 7) / 8, 1280 / blocks}));  // (of heads: all of them where the tokens alone fill the chip, up to eight by a wave in turn)
-    const int values = g.queries_only ? 0 : ((n + 62) / 32 + 3) / 4 * (int)g.kv_heads;
-    hipLaunchKernelGGL((few ? k_kv8_rows<TR, KL, VL, TAPS, 1> : k_kv8_rows<TR, KL, VL, TAPS, 4>), dim3((size_t)blocks * chunks + values), dim3(256), 0, s, c, (const TR *)rows, ld, pos, n, (TR *)q, ldq, blocks, chunks);
+    // values: a wave takes 32 positions where that fills the chip (16384 tokens 70.4 us with the read behind, 71.3 by eights), else eight (1531 tokens 7.0, 9.1 by 32)
+    auto groups = [&](int vp) { return g.queries_only ? 0 : ((n + 2 * vp - 2) / vp + 3) / 4 * (int)g.kv_heads; };  // (n tokens reach into (n + 2 vp - 2) / vp such pieces at most)
+    const bool many = !few && groups(32) >= 512;
+    auto fn = few ? k_kv8_rows<TR, KL, VL, TAPS, 1, 8> : many ? k_kv8_rows<TR, KL, VL, TAPS, 4, 32> : k_kv8_rows<TR, KL, VL, TAPS, 4, 8>;
+    hipLaunchKernelGGL(fn, dim3((size_t)blocks * chunks + groups(many ? 32 : 8)), dim3(256), 0, s, c, (const TR *)rows, ld, pos, n, (TR *)q, ldq, blocks, chunks);
     return hipGetLastError();
 }
 template <class TR, int TAPS>

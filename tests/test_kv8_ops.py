@@ -47,6 +47,12 @@ def test_written_bit_by_bit(hip, pkg, shape, n0, n, f32):
     assert u.rms_error(got[..., :t.dim], t.q[n0:]) < (1e-6 if f32 else 2.0 ** -8) and not got[..., t.dim:].any()
 
 
+@pytest.mark.parametrize("shape,n0,n", [((64, 64, 32, 32, 1), 5, 1100), ((30, 30, 24, 40, 2), 32, 2300), ((40, 40, 200, 200, 1), 19, 1700)])
+def test_many_tokens_of_many_heads(hip, pkg, shape, n0, n):
+    """values by pieces of 32 positions"""
+    test_written_bit_by_bit(hip, pkg, shape, n0, n, False)
+
+
 @pytest.mark.parametrize("f32", [True, False])
 @pytest.mark.parametrize("options", [dict(), dict(rot=16), dict(taps=3), dict(taps=5, rot=24), dict(taps=1, keys_as_values=True), dict(keys_as_values=True, rot=4)])
 @pytest.mark.parametrize("shape", [(6, 2, 24, 24, 1), (4, 2, 128, 128, 1), (2, 1, 200, 200, 1), (4, 2, 64, 100, 2)])

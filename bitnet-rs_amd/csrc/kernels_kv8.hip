@@ -860,7 +860,7 @@ __global__ __launch_bounds__(64 * W * G, NV > 8 || NK > 2 ? 1 : 2) void k_kv8_pr
             }
         }
         largest = rows_max(largest);
-        const int e = min(max(exponent_above(largest), -50), 100);
+        const int e = exponent_above(largest);
         qs[t] = is_finite(largest) ? kLog2e * power2(e - 12) : __builtin_nanf("");
 #pragma unroll
         for (int kk = 0; kk < KK; ++kk)

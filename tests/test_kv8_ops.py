@@ -231,6 +231,23 @@ def test_values_of_very_different_size(hip, pkg, spread):
         t.check(t.prompt(hip, qb, 0, n), t.want(u.host(qb).reshape(n, -1, t.dimp)[..., :t.dim], 0), *PROMPT)
 
 
+@pytest.mark.parametrize("up", [90, -90])
+def test_queries_and_keys_of_opposite_size(hip, pkg, up):
+    """powers of two that take each other away: the same scores"""
+    n = 200
+    t = kv.Attention(pkg, n, 4, 2, 64, 64, normed=False, f32=True)
+    heads = 4 * t.dimp
+    t.rows[:, :heads] *= np.float32(2.0 ** up)
+    t.rows[:, heads:heads + 2 * t.dimp] *= np.float32(2.0 ** -up)
+    t.convolved = t.rows[:, :t.channels].astype(f64)
+    t.q *= 2.0 ** up
+    t.fill(hip, 0, n - 1)
+    t.check(t.step(hip, n - 1), t.want(t.q[n - 1:], n - 1), STEP)
+    _, q = t.fill(hip, 0, n)
+    qb = as_bf16(q)
+    t.check(t.prompt(hip, qb, 0, n), t.want(u.host(qb).reshape(n, -1, t.dimp)[..., :t.dim], 0), *PROMPT)
+
+
 # ---- prompts ------------------------------------------------------------------------------------------------------------
 def prompted(hip, t, n0, n):
     if n0:

@@ -14,6 +14,7 @@
 #include <cfloat>
 
 #include "gqa.hpp"
+#include "kv8_schedule.hpp"
 
 namespace bitnet_hip {
 
@@ -822,6 +823,7 @@ constexpr float kWeightUp = 6.0f, kLazy = 8.0f;
 // Bound by both pipes of a SIMD: 8192 tokens of 20 heads on 5 of 128 columns, 344 GFLOP, take 393 us (0.87 PFLOP/s, a large product of f16 reaches 1.35; over a cache of bf16 k_gqa_prefill
 // takes 522); 509 tokens behind 20011 of 12 heads on 3 with two maps of 64 / 128 139 us (0.68), 130 tokens of 12 heads 12.3.  Phases one behind the other, two groups of four waves: 515,
 // 226, 11.5.
+// One barrier a tile: what is read and written between two of them is in kv8_schedule.hpp.
 // Wave 0 makes the values' factors two tiles ahead, wave 1 the keys' scales.  A value without a scale takes its key's away instead, so that only queries that see it lose theirs.
 // LDS of a tile: keys [maps][64][KS], values [columns][VS]; the 32 bytes behind a row of values hold the keys' scales (rows 16 s + 8 map .., s = 0
 // and 1 in turn), the factors (32 ..) and `above` (36).
@@ -910,13 +912,16 @@ __global__ __launch_bounds__(64 * W * G, NV > 8 || NK > 2 ? 1 : 2) void k_kv8_pr
     // The group's i-th tile; what lies past the last one is read from the last one, and all of it hidden.
     auto first_key = [&](int i) { return max(min(t_first + grp + G * i, n_tiles - 1), 0) * 64; };
     constexpr bool whole_keys = NKL * KR == MAPS * 64, whole_values = NVL * T == NV * 64;
-    auto fetch_keys = [&](int i) {  // (whole tiles: the capacity is a multiple of 64)
+    // which half of a tile a wave's j-th piece of the keys belongs to
+    auto half_of = [&](int j) { return (KR < 64 ? j * KR : wave * (64 / KC)) >> 5 & 1; };
+    constexpr Kv8Schedule ahead_by = kKv8Schedule;
+    auto keys_ahead = [&](int j) { return half_of(j) ? ahead_by.keys[1] : ahead_by.keys[0]; };
+    auto fetch_keys = [&](int i, int j) {  // (whole tiles: the capacity is a multiple of 64)
+        const int mp = MAPS == 1 ? 0 : (tid / KC + j * KR) >> 6 & 1;
+        if (whole_keys || tid / KC + j * KR < MAPS * 64) kreg[j] = *reinterpret_cast<const u32x4 *>(K + ((size_t)mp * p.capacity + first_key(i)) * dimp + koff[j]);
+    };
+    auto fetch_scales = [&](int i) {
         const int key0 = first_key(i);
-#pragma unroll
-        for (int j = 0; j < NKL; ++j) {
-            const int mp = MAPS == 1 ? 0 : (tid / KC + j * KR) >> 6 & 1;
-            if (whole_keys || tid / KC + j * KR < MAPS * 64) kreg[j] = *reinterpret_cast<const u32x4 *>(K + ((size_t)mp * p.capacity + key0) * dimp + koff[j]);
-        }
         if (wave == 1) {
             const bool in = key0 + lane < n_ctx;  // (a position past the portion may hold anything)
 #pragma unroll
@@ -950,8 +955,12 @@ __global__ __launch_bounds__(64 * W * G, NV > 8 || NK > 2 ? 1 : 2) void k_kv8_pr
     auto store_keys = [&](int i, int u) {
         uint8_t *dst = lk + (i & 1) * TILE;
         const int j = u >> 1;
-        if (whole_keys || tid / KC + j * KR < MAPS * 64) *reinterpret_cast<f16x8 *>(dst + kw[j] + (u & 1) * 16) = u & 1 ? eight_raised(kreg[j].z, kreg[j].w) : eight_raised(kreg[j].x, kreg[j].y);
-        if (u == 2 * NKL - 1 && wave == 1)
+        if (whole_keys || tid / KC + j * KR < MAPS * 64)
+            *reinterpret_cast<f16x8 *>(dst + kw[j] + (u & 1) * 16) = u & 1 ? eight_raised(kreg[j].z, kreg[j].w) : eight_raised(kreg[j].x, kreg[j].y);
+    };
+    auto store_scales = [&](int i) {
+        uint8_t *dst = lk + (i & 1) * TILE;
+        if (wave == 1)
 #pragma unroll
             for (int mp = 0; mp < MAPS; ++mp)
                 *reinterpret_cast<float *>(dst + PAD + ((i >> 1 & 1) * 16 + 8 * mp + (lane >> 3)) * VS + (lane & 7) * 4) = vnan == vnan ? kscale[mp] : vnan;
@@ -968,13 +977,19 @@ __global__ __launch_bounds__(64 * W * G, NV > 8 || NK > 2 ? 1 : 2) void k_kv8_pr
             *reinterpret_cast<f16x8 *>(lk + (i & 1) * TILE + vw[j] + (u & 1) * 16 * VS) = (u & 1 ? eight_f16(vreg[j].z, vreg[j].w) : eight_f16(vreg[j].x, vreg[j].y)) * factor[j];
     };
     const int steps = (n_tiles - t_first + G - 1) / G;
-    // keys of tiles 0 and 1, values of tile 0, factors of tiles 0 and 1
-    fetch_keys(0), fetch_values(0), fetch_factors(0);
+    // what the first iteration finds: keys 0 .. 31 of tiles 0 and 1 and 32 .. 63 of tile 0, their tiles' scales, values of tile 0, factors of tiles 0 and 1
+    static_assert(ahead_by.keys[0] == 2 && ahead_by.keys[1] == 1 && ahead_by.scales == 2 && ahead_by.values == 1 && ahead_by.factors == 2 && ahead_by.slots == 2, "what the prologue leaves");
+#pragma unroll
+    for (int j = 0; j < NKL; ++j) fetch_keys(0, j);
+    fetch_scales(0), fetch_values(0), fetch_factors(0);
     publish(0);
     fetch_factors(1);
 #pragma unroll
     for (int u = 0; u < 2 * NKL; ++u) store_keys(0, u);
-    fetch_keys(1);
+    store_scales(0);
+#pragma unroll
+    for (int j = 0; j < NKL; ++j) fetch_keys(1, j);
+    fetch_scales(1);
     __syncthreads();
     publish(1);
     fetch_factors(2);
@@ -983,8 +998,13 @@ __global__ __launch_bounds__(64 * W * G, NV > 8 || NK > 2 ? 1 : 2) void k_kv8_pr
     for (int u = 0; u < 2 * NVL; ++u) store_values(0, u);
     fetch_values(1);
 #pragma unroll
-    for (int u = 0; u < 2 * NKL; ++u) store_keys(1, u);
-    fetch_keys(2);
+    for (int u = 0; u < 2 * NKL; ++u)
+        if (half_of(u >> 1) == 0) store_keys(1, u);
+    store_scales(1);
+#pragma unroll
+    for (int j = 0; j < NKL; ++j)
+        if (half_of(j) == 0) fetch_keys(2, j);
+    fetch_scales(2);
     // Scores go by halves of a tile (32 keys): of the half at hand and of the next one, times their keys' scales, in units of qs, which holds log2(e).
     f32x4 s0[2][SLOTS], s1[2][SLOTS];
     float mx[SLOTS];  // the largest of the lane's
@@ -1056,7 +1076,7 @@ __global__ __launch_bounds__(64 * W * G, NV > 8 || NK > 2 ? 1 : 2) void k_kv8_pr
                 for (int v = 0; v < NV; ++v) o[v][t] *= al * down;
             }
         }
-        if (half == 0) read_factors(i + 1);
+        if (half == 0) read_factors(i + ahead_by.values);
         u32x4 w[SLOTS];
         {
             f16x8 k[KREADS];
@@ -1093,21 +1113,25 @@ __global__ __launch_bounds__(64 * W * G, NV > 8 || NK > 2 ? 1 : 2) void k_kv8_pr
                 for (int u = j * 4 / NV; u < (j + 1) * 4 / NV; ++u) scaled(next, ni, other, u, ahead);
                 constexpr int VP = 2 * NVL, KP = 2 * NKL;
 #pragma unroll
-                for (int u = j * VP / NV; half == 0 && u < (j + 1) * VP / NV; ++u) store_values(i + 1, u);
+                for (int u = j * VP / NV; half == 0 && u < (j + 1) * VP / NV; ++u) store_values(i + ahead_by.values, u);
 #pragma unroll
-                for (int u = j * KP / NV; half == 1 && u < (j + 1) * KP / NV; ++u) store_keys(i + 2, u);
+                for (int u = j * KP / NV; half == 1 && u < (j + 1) * KP / NV; ++u) store_keys(i + keys_ahead(u >> 1), u);
             }
-            if (half == 0)
-                fetch_values(i + 2);
-            else
-                fetch_keys(i + 3);
+            if (half == 0) {
+                fetch_values(i + ahead_by.values + 1);
+            } else {
+                store_scales(i + ahead_by.scales);
+#pragma unroll
+                for (int u = 0; u < NKL; ++u) fetch_keys(i + keys_ahead(u) + 1, u);
+                fetch_scales(i + ahead_by.scales + 1);
+            }
         }
         __builtin_amdgcn_sched_barrier(0);
     };
     for (int i = 0; i < steps; ++i) {
         __syncthreads();
-        publish(i + 2);
-        fetch_factors(i + 3);
+        publish(i + ahead_by.factors);
+        fetch_factors(i + ahead_by.factors + 1);
         const int need = __builtin_amdgcn_readfirstlane(*reinterpret_cast<const int *>(lk + (i & 1) * TILE + PAD + 36 * VS + (i >> 1 & 1) * 4));
         step(i, 0, need, s0, s1);
         step(i, 1, need, s1, s0);

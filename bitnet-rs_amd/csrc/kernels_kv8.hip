@@ -360,10 +360,9 @@ __global__ __launch_bounds__(256) void k_kv8_read(Kv8 c, int first, int n, TO *k
     const Gqa &p = c.g;
     const int tid = threadIdx.x, nk = keys ? (int)(p.kv_heads * p.maps) : 0, dimp = (int)p.dimp, vdimp = (int)p.vdimp;
     if ((int)blockIdx.y < nk) {
-        const int pieces = dimp >> 4, i = blockIdx.x * 256 + tid, t = i / pieces;
-        if (t >= n) return;
+        const int pieces = dimp >> 4, t_here = tid / pieces, at = (tid - t_here * pieces) * 16, t = (int)blockIdx.x * (256 / pieces) + t_here;  // (whole rows: pieces of all of them may be more than 2^31)
+        if (t_here >= 256 / pieces || t >= n) return;
         const size_t row = (size_t)blockIdx.y * p.capacity + first + t;
-        const int at = (i - t * pieces) * 16;
         const u32x4 v = *reinterpret_cast<const u32x4 *>((const int8_t *)p.kcache + row * dimp + at);
         const float s = c.k_scale[row];
         TO *dst = keys + ((size_t)blockIdx.y * n + t) * dimp + at;
@@ -391,7 +390,7 @@ __global__ __launch_bounds__(256) void k_kv8_read(Kv8 c, int first, int n, TO *k
 hipError_t launch_kv8_read(const Kv8 &c, int first, int n, void *keys, void *values, int f32, hipStream_t s) {
     const Gqa &g = c.g;
     const int rows = (int)((keys ? g.kv_heads * g.maps : 0) + (values ? g.kv_heads : 0));
-    const size_t blocks = std::max(keys ? ((size_t)n * (g.dimp / 16) + 255) / 256 : (size_t)1, values ? ((size_t)n + 62) / 32 : (size_t)1);
+    const size_t each = 256 / (g.dimp / 16), blocks = std::max(keys ? (n + each - 1) / each : (size_t)1, values ? ((size_t)n + 62) / 32 : (size_t)1);
     if (f32)
         hipLaunchKernelGGL(k_kv8_read<float>, dim3(blocks, rows), dim3(256), 0, s, c, first, n, (float *)keys, (float *)values);
     else

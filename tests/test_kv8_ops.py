@@ -454,3 +454,24 @@ def test_caches_past_two_gigabytes(hip, pkg):
     hip.kv8_step_dev(t.attn, big.ks, big.vs, u.dev_f32(t.rows[639]), at, scratch)
     hip.gqa_merge_dev(t.attn, at, 0, 1, scratch, out, heads * 256, False)
     assert u.rms_error(u.host(out), u.host(small.step(hip, 639))) < 2 * STEP
+
+
+def test_more_than_two_to_the_31_pieces_read_back(hip, pkg):
+    """a cache whose keys are more than 2^31 pieces of sixteen bytes, read in one call"""
+    import torch
+
+    n = 2 ** 27 + 72
+    if torch.cuda.mem_get_info()[0] < 3.3 * 256 * n:
+        pytest.skip("wants 110 GB")
+    cap = u.up_to(n, 128)
+    keys, scales = torch.zeros(cap, 256, dtype=torch.int8, device="cuda"), torch.zeros(cap, device="cuda")
+    some = torch.tensor([0, 1, 15, 16, 17, 255, 4099, 2 ** 26 + 3, 2 ** 27 - 1, 2 ** 27, 2 ** 27 + 1, n - 17, n - 1], device="cuda")
+    numbers = torch.randint(-127, 128, (len(some), 256), generator=torch.Generator(device="cuda").manual_seed(0), device="cuda", dtype=torch.int8)
+    keys[some], scales[some] = numbers, torch.arange(1, len(some) + 1, device="cuda") * 0.5
+    attn = pkg.Gqa(1, 1, 1, 256, 256, 256, 256, cap, 1e-5, 0.0, 1.0, 0, 0, scales.data_ptr(), keys.data_ptr(), keys.data_ptr())
+    out = torch.full((n + 1, 256), 3, dtype=torch.bfloat16, device="cuda")
+    hip.kv8_read_dev(attn, scales, scales, 0, n, out, None, False)
+    assert bool((out[some].float() == (numbers.float() * scales[some, None]).bfloat16().float()).all()) and bool((out[n] == 3).all())
+    assert int(torch.count_nonzero(out[:n].view(torch.int16).view(torch.int64))) <= len(some) * 64
+    del keys, out
+    torch.cuda.empty_cache()

@@ -218,6 +218,7 @@ static int check_kv8(const bitnet_hip_gqa *a, const float *k_scale, const float 
     BH_REQUIRE(k_scale && v_scale && (((uintptr_t)a->kcache | (uintptr_t)a->vcache | (uintptr_t)k_scale | (uintptr_t)v_scale) & 15) == 0, "kv8: caches and scales on 16 bytes");
     return 0;
 }
+constexpr size_t kKv8Rows = size_t(1) << 30;  // rows of a prompt's launch (queries times heads): it counts them in 32 bits
 static Kv8 kv8_of(const bitnet_hip_gqa *a, const float *k_scale, const float *v_scale) {
     Kv8 c;
     c.g = *a, c.k_scale = const_cast<float *>(k_scale), c.v_scale = const_cast<float *>(v_scale);
@@ -262,7 +263,7 @@ int bitnet_hip_kv8_step_dev(const bitnet_hip_gqa *a, float *k_scale, float *v_sc
 }
 
 size_t bitnet_hip_kv8_prefill_scratch_bytes(const bitnet_hip_gqa *a, size_t n_ctx, size_t nq) {
-    if (!a || check_gqa(a) != 0 || nq == 0 || nq > n_ctx || n_ctx > a->capacity || !gqa_supported((int)a->dimp, (int)a->vdimp)) return 0;
+    if (!a || check_gqa(a) != 0 || nq == 0 || nq > n_ctx || n_ctx > a->capacity || !gqa_supported((int)a->dimp, (int)a->vdimp) || nq * a->heads > kKv8Rows) return 0;
     return kv8_prefill_floats(*a, (int)n_ctx, (int)nq) * sizeof(float);
 }
 
@@ -273,6 +274,7 @@ int bitnet_hip_kv8_prefill_dev(const bitnet_hip_gqa *a, const float *k_scale, co
     BH_REQUIRE(q && out && nq > 0 && nq <= n_ctx && n_ctx <= a->capacity && ldq % 8 == 0 && ldq >= a->heads * a->maps * a->dimp && ldo % 4 == 0 && ldo >= a->heads * a->vdimp &&
                    (uintptr_t)q % 16 == 0 && (uintptr_t)out % 8 == 0,
                "kv8_prefill: bad arguments");
+    BH_REQUIRE(nq * a->heads <= kKv8Rows, "kv8_prefill: %zu queries of %zu heads are too many for one launch", nq, a->heads);
     BH_CHECK_DIMS(nq, ldq);
     const size_t bytes = scratch || kv8_prefill_wants_records(*a) ? kv8_prefill_floats(*a, (int)n_ctx, (int)nq) * sizeof(float) : 0;
     BH_REQUIRE(bytes == 0 || scratch, "kv8_prefill: two maps of heads of more than 128 columns want scratch");

@@ -76,3 +76,11 @@ def test_order_of_the_values():
 def test_numbers_of_a_vector():
     n, s = kv.numbers_of([[1.0, -2.0, 0.5, 0.0], [0, 0, 0, 0], [np.nan, 1, 2, 3], [127, 0.5, 1.5, -2.5]])
     assert n.tolist() == [[64, -127, 32, 0], [0, 0, 0, 0], [0, 0, 0, 0], [127, 0, 2, -2]] and s[1] == 0 and np.isnan(s[2]) and s[3] == 1
+
+
+def test_more_rows_than_a_prompts_launch_can_count(built):
+    hip = built.load()
+    g = built.Gqa(16384, 1, 1, 16, 32, 16, 32, 2 ** 17, 1e-5, 0.1, 0.9, 8, 8, 8, 16, 16)
+    with pytest.raises(built.BitNetHipError, match="too many for one launch"):
+        hip.kv8_prefill_dev(g, 16, 16, 16, 16384 * 32, 2 ** 17, 2 ** 17, 16, 16384 * 32)
+    assert hip.kv8_prefill_scratch_bytes(g, 2 ** 17, 2 ** 17) == 0

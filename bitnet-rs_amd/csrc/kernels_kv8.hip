@@ -19,6 +19,7 @@
 namespace bitnet_hip {
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
@@ -51,8 +52,8 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
     return r;
 }
-// the least E with |v| < 2^E (v = 0: -100)
-__device__ __forceinline__ int exponent_above(float v) { return v > 0.f ? max(__builtin_amdgcn_frexp_expf(v), -100) : -100; }
+// the least E with |v| < 2^E (v = 0: `least`, which is the least it gives)
+__device__ __forceinline__ int exponent_above(float v, int least) { return v > 0.f ? max(__builtin_amdgcn_frexp_expf(v), least) : least; }
 __device__ __forceinline__ float power2(int e) { return __builtin_amdgcn_ldexpf(1.0f, e); }
 
 // How a vector of an 8-bit cache is held: whole numbers -127 .. 127 and one scale.  The scale stays 32 bits wide.  What is smaller than 1.5e-36 throughout counts as zero (its scale would
@@ -651,7 +652,7 @@ __global__ __launch_bounds__(256, step_held(NK, NV, MAPS)) void k_kv8_step(Kv8St
 #pragma unroll
                 for (int e = 0; e < 4; ++e) sv[t][e] = seen(t, e) ? sv[t][e] : 0.f;
         const float largest = fmaxf(fmaxf(fmaxf(sv[0][0], sv[0][1]), fmaxf(sv[0][2], sv[0][3])), fmaxf(fmaxf(sv[1][0], sv[1][1]), fmaxf(sv[1][2], sv[1][3])));
-        const int need = __builtin_amdgcn_readfirstlane(exponent_above(rows_max(largest)));
+        const int need = __builtin_amdgcn_readfirstlane(exponent_above(rows_max(largest), -100));
         if (need > above) {
             const float down = power2(max(above - need, -140));
 #pragma unroll
@@ -807,25 +808,29 @@ hipError_t launch_kv8_step(const Kv8 &c, const GqaStep &a, hipStream_t s) {
 
 // ---- prompt -----------------------------------------------------------------------------------------------------------
 constexpr int kv8_tile_bytes(int nk, int nv, int maps) { return maps * 64 * (nk * 128 + 32) + nv * 16 * (64 * 2 + 32); }
-// A weight is exp2(score - m) times 2^kWeightUp, m being a maximum that follows the largest score once that is kLazy above it: at most 2^14.
-constexpr float kWeightUp = 6.0f, kLazy = 8.0f;
+// A share is a weight, exp2(score - m) times 2^kWeightUp, times its value's factor, the scale without the power of two that the largest scale so far needs.  m follows the exponent of a query's
+// largest share (score plus the factor's exponent, of what the query sees) once that may be kLazy above it: shares are at most 2^14 and a query's largest one is 2^6 or more, so that an f16
+// holds 11 bits of all that are 2^-20 of the largest, whatever lies at positions that the query does not see or weigh.  (A weight alone, of a small value, may be larger: sums are f32.)
+// Factors count as 2^kBelow at least in that, which keeps sums finite: scales down to 2^-64 of the largest one up to the portion's end keep their bits.
+constexpr float kWeightUp = 6.0f, kLazy = 8.0f, kLittle = 2.0f;
+constexpr int kLeast = -126, kBelow = -64;
 
 // One workgroup: the rows of W waves, a row being a query of one head; the heads that share keys and values are neighbours among the rows (row r: query r / group, head r % group of
 // the kv head).  A wave holds two slots of 16 rows: both maps of one set of rows, or two sets of the only map.  Key tiles of 64 (every map's) and the values of a tile are staged
 // through registers into LDS.  G = 2: two such groups of W waves share the keys of the same rows, tile by tile in turn, and meet in LDS at the end.  records: gridDim.y workgroups
 // share a block's tiles of keys, in stretches (launch_gqa_merge_parts).  MAPS = 1 with two maps, whose keys together find no room in LDS: gridDim.z is the map, with records.
 // In LDS keys are their numbers + 1152 as f16 (exact; a row's sum times 1152 is what its scores start from), and so is a query of bf16 times a power of two: scores are exact but
-// for the f32 sums, a key's scale meets them in f32.  Values are number times scale, brought under 2^15 by a power of two that holds for the group's tiles so far (`above`; o is
-// times 2^(8 - above)): a rounding of 2^-12 like that of the weights.  The sum of the weights is one more row of the products (ones times the same f16 weights).
+// for the f32 sums, a key's scale meets them in f32.  Values are their numbers (exact in f16), and a weight times its value's factor is rounded to f16 once, to the nearest
+// (2^-11 of it at most, 1.5e-4 of an output that is rounded to 2^-8 afterwards; f16 pairs would double these products).
 // The products of a SIMD's two waves and their vector instructions take about the same time, and as phases of their own they add up: hence the next tile's scores are made among
 // this tile's exponentials, and this tile's outputs among the staging of the tiles to come.
-// Bound by both pipes of a SIMD: 8192 tokens of 20 heads on 5 of 128 columns, 344 GFLOP, take 393 us (0.87 PFLOP/s, a large product of f16 reaches 1.35; over a cache of bf16 k_gqa_prefill
-// takes 522); 509 tokens behind 20011 of 12 heads on 3 with two maps of 64 / 128 139 us (0.68), 130 tokens of 12 heads 12.3.  Phases one behind the other, two groups of four waves: 515,
+// Bound by both pipes of a SIMD: 8192 tokens of 20 heads on 5 of 128 columns, 344 GFLOP, take 420 us (0.82 PFLOP/s, a large product of f16 reaches 1.35; over a cache of bf16 k_gqa_prefill
+// takes 522); 509 tokens behind 20011 of 12 heads on 3 with two maps of 64 / 128 148 us (0.64), 130 tokens of 12 heads 12.6.  Phases one behind the other, two groups of four waves: 515,
 // 226, 11.5.
 // One barrier a tile: what is read and written between two of them is in kv8_schedule.hpp.
-// Wave 0 makes the values' factors two tiles ahead, wave 1 the keys' scales.  A value without a scale takes its key's away instead, so that only queries that see it lose theirs.
+// Wave 0 makes the values' factors a tile ahead, wave 1 the keys' scales two.  A value without a scale takes its key's away instead, so that only queries that see it lose theirs.
 // LDS of a tile: keys [maps][64][KS], values [columns][VS]; the 32 bytes behind a row of values hold the keys' scales (rows 16 s + 8 map .., s = 0
-// and 1 in turn), the factors (32 ..) and `above` (36).
+// and 1 in turn), the factors (32 ..) and their exponents (40).
 // FAR: with a distance penalty, gates per column, or both.
 template <int NK, int NV, int MAPS, bool FAR, int G, int W>
 __global__ __launch_bounds__(64 * W * G, NV > 8 || NK > 2 ? 1 : 2) void k_kv8_prefill(Kv8 c, const uint16_t *Q, size_t ldq, int n_ctx, int nq, uint16_t *out, size_t ldo, int n_qb, float *records) {
@@ -841,10 +846,10 @@ __global__ __launch_bounds__(64 * W * G, NV > 8 || NK > 2 ? 1 : 2) void k_kv8_pr
     const int pos0 = n_ctx - nq, row0 = qb * W * QW, rw = row0 + wave * QW, last = nq - 1;
     const int q_lo = min(rw / group, last), q_hi = min((rw + QW - 1) / group, last), q_first = row0 / group, q_last = min((row0 + W * QW - 1) / group, last);
     f16x8 qf[SLOTS][KK];
-    float qs[SLOTS], raised[SLOTS], m[SLOTS];
+    float qs[SLOTS], raised[SLOTS], m[SLOTS], l[SLOTS];
     FarPenalty far[SLOTS / MAPS];
     int qpos[SLOTS], qfirst[SLOTS], head[SLOTS / MAPS];
-    f32x4 o[NV][SLOTS], l[SLOTS];
+    f32x4 o[NV][SLOTS];
 #pragma unroll
     for (int t = 0; t < SLOTS; ++t) {
         const int at = rw + t / MAPS * 16 + r16, qi = min(at / group, last), h = kv * group + at % group, map = alone + t % MAPS;
@@ -861,7 +866,7 @@ __global__ __launch_bounds__(64 * W * G, NV > 8 || NK > 2 ? 1 : 2) void k_kv8_pr
             }
         }
         largest = rows_max(largest);
-        const int e = exponent_above(largest);
+        const int e = exponent_above(largest, -100);
         qs[t] = is_finite(largest) ? kLog2e * power2(e - 12) : __builtin_nanf("");
 #pragma unroll
         for (int kk = 0; kk < KK; ++kk)
@@ -874,18 +879,16 @@ __global__ __launch_bounds__(64 * W * G, NV > 8 || NK > 2 ? 1 : 2) void k_kv8_pr
         // (finite: with chunks a tile may hold no key that a query sees)
         m[t] = -1e30f;
         if (FAR && MAPS == 1) far[t] = far_penalty(p, h), far[t].weight *= kLog2e;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) l[t][i] = 0.f;
+        l[t] = 0.f;
 #pragma unroll
         for (int v = 0; v < NV; ++v) o[v][t] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    int above = -60;
     const int8_t *K = (const int8_t *)p.kcache + (size_t)(kv * maps + alone) * p.capacity * dimp, *V = (const int8_t *)p.vcache + (size_t)kv * vdimp * p.capacity;
     const float *KSC = c.k_scale + (size_t)(kv * maps + alone) * p.capacity, *VSC = c.v_scale + (size_t)kv * p.capacity;
     // keys: a row of the tile by KC neighbouring threads; row p of 32 in LDS is key 8 (p >> 2 & 3) + 4 (p >> 4) + (p & 3)
     u32x4 kreg[NKL], vreg[NVL];
     float kscale[MAPS], vscale = 0.f, vnan = 0.f;
-    int kw[NKL], vw[NVL], voff[NVL], vf[NVL];
+    int kw[NKL], vw[NVL], voff[NVL];
     unsigned koff[NKL];
 #pragma unroll
     for (int j = 0; j < NKL; ++j) {
@@ -898,7 +901,6 @@ __global__ __launch_bounds__(64 * W * G, NV > 8 || NK > 2 ? 1 : 2) void k_kv8_pr
         const int i = tid + T * j, half = i / (NV * 32) & 1, rem = i % (NV * 32), key = half * 32 + (rem & 3) * 8;
         vw[j] = KB + ((rem >> 6) * 32 + (rem >> 2 & 15)) * VS + key * 2;
         voff[j] = (rem >> 6) * 32 < vdimp ? half * vdimp * 32 + rem * 16 : -1;
-        vf[j] = PAD + (32 + (key >> 4)) * VS + (key & 8) * 2;
         vreg[j] = u32x4{0u, 0u, 0u, 0u};
     }
     int t_first = gqa_first(p, pos0 + q_first) >> 6, n_tiles = (pos0 + q_last) / 64 + 1;
@@ -940,14 +942,15 @@ __global__ __launch_bounds__(64 * W * G, NV > 8 || NK > 2 ? 1 : 2) void k_kv8_pr
             vscale = key0 + lane < n_ctx ? VSC[key0 + lane] : 0.f;
         }
     };
-    int highest = -60;
-    auto publish = [&](int i) {  // the factors of tile i
+    int highest = kLeast;
+    auto publish = [&](int i) {  // the factors of tile i, the exponent that they are without, and how far below it they all are
         if (wave == 0) {
             const float v = fmaxf(vscale, 0.f);
-            highest = max(highest, __builtin_amdgcn_readfirstlane(min(exponent_above(rows_max(row_max(v))), 126)));
-            uint8_t *dst = lk + (i & 1) * TILE + PAD;
-            *reinterpret_cast<_Float16 *>(dst + (32 + (lane >> 4)) * VS + (lane & 15) * 2) = (_Float16)__builtin_amdgcn_ldexpf(v, 8 - highest);
-            if (lane == 0) *reinterpret_cast<int *>(dst + 36 * VS + (i >> 1 & 1) * 4) = highest;
+            const int here = __builtin_amdgcn_readfirstlane(exponent_above(rows_max(row_max(v)), kLeast));
+            highest = max(highest, here);
+            uint8_t *dst = lk + (i & 1) * TILE + PAD + 32 * VS;
+            *reinterpret_cast<float *>(dst + (lane >> 3) * VS + (lane & 7) * 4) = __builtin_amdgcn_ldexpf(v, -highest);
+            if (lane == 0) *reinterpret_cast<int2 *>(dst + 8 * VS) = int2{highest, max(here - highest, kBelow)};
         }
     };
     // stores go by pieces of eight numbers a thread, 2 NKL and 2 NVL of them
@@ -964,20 +967,14 @@ __global__ __launch_bounds__(64 * W * G, NV > 8 || NK > 2 ? 1 : 2) void k_kv8_pr
             for (int mp = 0; mp < MAPS; ++mp)
                 *reinterpret_cast<float *>(dst + PAD + ((i >> 1 & 1) * 16 + 8 * mp + (lane >> 3)) * VS + (lane & 7) * 4) = vnan == vnan ? kscale[mp] : vnan;
     };
-    f16x8 factor[NVL];
-    auto read_factors = [&](int i) {
-#pragma unroll
-        for (int j = 0; j < NVL; ++j)
-            if (whole_values || tid + T * j < NV * 64) factor[j] = *reinterpret_cast<const f16x8 *>(lk + (i & 1) * TILE + vf[j]);
-    };
     auto store_values = [&](int i, int u) {
         const int j = u >> 1;
         if (whole_values || tid + T * j < NV * 64)
-            *reinterpret_cast<f16x8 *>(lk + (i & 1) * TILE + vw[j] + (u & 1) * 16 * VS) = (u & 1 ? eight_f16(vreg[j].z, vreg[j].w) : eight_f16(vreg[j].x, vreg[j].y)) * factor[j];
+            *reinterpret_cast<f16x8 *>(lk + (i & 1) * TILE + vw[j] + (u & 1) * 16 * VS) = u & 1 ? eight_f16(vreg[j].z, vreg[j].w) : eight_f16(vreg[j].x, vreg[j].y);
     };
     const int steps = (n_tiles - t_first + G - 1) / G;
-    // what the first iteration finds: keys 0 .. 31 of tiles 0 and 1 and 32 .. 63 of tile 0, their tiles' scales, values of tile 0, factors of tiles 0 and 1
-    static_assert(ahead_by.keys[0] == 2 && ahead_by.keys[1] == 1 && ahead_by.scales == 2 && ahead_by.values == 1 && ahead_by.factors == 2 && ahead_by.slots == 2, "what the prologue leaves");
+    // what the first iteration finds: keys 0 .. 31 of tiles 0 and 1 and 32 .. 63 of tile 0, their tiles' scales, values and factors of tile 0
+    static_assert(ahead_by.keys[0] == 2 && ahead_by.keys[1] == 1 && ahead_by.scales == 2 && ahead_by.values == 1 && ahead_by.factors == 1 && ahead_by.slots == 2, "what the prologue leaves");
 #pragma unroll
     for (int j = 0; j < NKL; ++j) fetch_keys(0, j);
     fetch_scales(0), fetch_values(0), fetch_factors(0);
@@ -990,9 +987,6 @@ __global__ __launch_bounds__(64 * W * G, NV > 8 || NK > 2 ? 1 : 2) void k_kv8_pr
     for (int j = 0; j < NKL; ++j) fetch_keys(1, j);
     fetch_scales(1);
     __syncthreads();
-    publish(1);
-    fetch_factors(2);
-    read_factors(0);
 #pragma unroll
     for (int u = 0; u < 2 * NVL; ++u) store_values(0, u);
     fetch_values(1);
@@ -1034,11 +1028,9 @@ __global__ __launch_bounds__(64 * W * G, NV > 8 || NK > 2 ? 1 : 2) void k_kv8_pr
     for (int j = 0; j < KREADS; ++j) key_products(key_operand(lk, 0, j), j, s0);
 #pragma unroll
     for (int j = 0; j < 4; ++j) scaled(lk, 0, 0, j, s0);
-    f16x8 one;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) one[i] = (_Float16)1.0f;
+    int above = __builtin_amdgcn_readfirstlane(*reinterpret_cast<const int *>(lk + PAD + 40 * VS));
     // half `half` of tile i, its scores in s; the half behind it, of tile ni, into ahead
-    auto step = [&](int i, int half, int need, f32x4 (&s)[2][SLOTS], f32x4 (&ahead)[2][SLOTS]) __attribute__((always_inline)) {
+    auto step = [&](int i, int half, int2 need, f32x4 (&s)[2][SLOTS], f32x4 (&ahead)[2][SLOTS]) __attribute__((always_inline)) {
         const int key0 = (t_first + grp + G * i) * 64 + half * 32, ni = i + half, other = half ^ 1;
         const uint8_t *here = lk + (i & 1) * TILE, *next = lk + (ni & 1) * TILE;
         if (key0 + 31 > min(pos0 + q_lo, end) || key0 < w_last || (FAR && p.far_weight))  // (the diagonal or what lies past the last tile; an earlier chunk of some of the queries)
@@ -1057,27 +1049,45 @@ __global__ __launch_bounds__(64 * W * G, NV > 8 || NK > 2 ? 1 : 2) void k_kv8_pr
                     }
             }
         float c2[SLOTS];
-        bool grows = need > above;
+        auto factors = [&](int kt) { return *reinterpret_cast<const f32x4 *>(here + PAD + (32 + half * 4 + g) * VS + kt * 16); };
+        bool grows = need.x > above;
+        const float most = kLazy - (float)need.y;
 #pragma unroll
         for (int t = 0; t < SLOTS; ++t) {
             c2[t] = FAR && p.far_weight ? 1.0f : qs[t];
-            grows = grows || mx[t] * c2[t] > m[t] + kLazy;
+            grows = grows || mx[t] * c2[t] > m[t] + most;
         }
         if (__any(grows)) {
-            const float down = power2(min(above - need, 0));
-            above = max(above, need);
+            const int less = max(need.x - above, 0);  // (factors from here on are 2^-less of what they would have been)
+            above = max(above, need.x);
+            float e[2][4];
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) e[kt][i] = (float)exponent_above(factors(kt)[i], kBelow);
 #pragma unroll
             for (int t = 0; t < SLOTS; ++t) {
-                const float largest = rows_max(mx[t]) * c2[t], to = largest > m[t] + kLazy ? largest : m[t], al = __builtin_amdgcn_exp2f(m[t] - to);
+                float largest = -INFINITY;
+#pragma unroll
+                for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) largest = fmaxf(largest, fmaf(s[kt][t][i], c2[t], e[kt][i]));
+                largest = rows_max(largest);
+                // m moves with the factors as far as the sum has room, so that a query that does not see what is large keeps its bits; the outputs take the rest
+                const float total = rows_sum(l[t]);
+                const int moved = total > 0.f ? min(less, max(100 - __builtin_amdgcn_frexp_expf(total), 0)) : min(less, 100);
+                const float from = m[t] - (float)moved, to = largest > from + kLittle ? largest : from, al = __builtin_amdgcn_exp2f(from - to), down = power2(moved - less);
                 m[t] = to;
-                l[t] *= al;
+                l[t] *= al * power2(moved);
 #pragma unroll
                 for (int v = 0; v < NV; ++v) o[v][t] *= al * down;
             }
         }
-        if (half == 0) read_factors(i + ahead_by.values);
         u32x4 w[SLOTS];
         {
+            // (scores in place and factors read again: what the compiler would keep of both across the branch costs up to 160 registers)
+            asm volatile("" : "+v"(s[0][0]), "+v"(s[0][1]), "+v"(s[1][0]), "+v"(s[1][1])::"memory");
+            const f32x4 vs[2] = {factors(0), factors(1)};
             f16x8 k[KREADS];
 #pragma unroll
             for (int j = 0; j < AHEAD; ++j) k[j] = key_operand(next, other, j);
@@ -1088,10 +1098,11 @@ __global__ __launch_bounds__(64 * W * G, NV > 8 || NK > 2 ? 1 : 2) void k_kv8_pr
                 key_products(k[j], j, ahead);
 #pragma unroll
                 for (int u = j * 8 / KREADS; u < (j + 1) * 8 / KREADS; ++u) {  // two weights
-                    const int t = u >> 2, e = u & 3;
+                    const int t = u % SLOTS, e = u / SLOTS;
                     const float off = kWeightUp - m[t];
                     const float a = __builtin_amdgcn_exp2f(fmaf(s[e >> 1][t][2 * e & 3], c2[t], off)), b = __builtin_amdgcn_exp2f(fmaf(s[e >> 1][t][(2 * e & 3) + 1], c2[t], off));
-                    w[t][e] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));  // (cut off, in the sum as in the products)
+                    l[t] += a + b;
+                    w[t][e] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a * vs[e >> 1][2 * e & 3], b * vs[e >> 1][(2 * e & 3) + 1]}), f16x2));
                 }
             }
         }
@@ -1100,8 +1111,6 @@ __global__ __launch_bounds__(64 * W * G, NV > 8 || NK > 2 ? 1 : 2) void k_kv8_pr
             f16x8 v[NV];
 #pragma unroll
             for (int j = 0; j < AHEAD; ++j) v[j] = value_operand(here, half, j);
-#pragma unroll
-            for (int t = 0; t < SLOTS; ++t) l[t] = mfma_f16(one, __builtin_bit_cast(f16x8, w[t]), l[t]);
 #pragma unroll
             for (int j = 0; j < NV; ++j) {
                 __builtin_amdgcn_sched_barrier(0);
@@ -1131,15 +1140,16 @@ __global__ __launch_bounds__(64 * W * G, NV > 8 || NK > 2 ? 1 : 2) void k_kv8_pr
         __syncthreads();
         publish(i + ahead_by.factors);
         fetch_factors(i + ahead_by.factors + 1);
-        const int need = __builtin_amdgcn_readfirstlane(*reinterpret_cast<const int *>(lk + (i & 1) * TILE + PAD + 36 * VS + (i >> 1 & 1) * 4));
+        const int2 both = *reinterpret_cast<const int2 *>(lk + (i & 1) * TILE + PAD + 40 * VS);
+        const int2 need{__builtin_amdgcn_readfirstlane(both.x), __builtin_amdgcn_readfirstlane(both.y)};
         step(i, 0, need, s0, s1);
         step(i, 1, need, s1, s0);
     }
     float sum[SLOTS];
 #pragma unroll
     for (int t = 0; t < SLOTS; ++t) {
-        const float back = power2(above - 8 - (int)kWeightUp);
-        sum[t] = l[t].x * power2(-(int)kWeightUp);
+        const float back = power2(above - (int)kWeightUp);
+        sum[t] = rows_sum(l[t]) * power2(-(int)kWeightUp);
 #pragma unroll
         for (int v = 0; v < NV; ++v) o[v][t] *= back;
     }

@@ -475,3 +475,72 @@ def test_more_than_two_to_the_31_pieces_read_back(hip, pkg):
     assert int(torch.count_nonzero(out[:n].view(torch.int16).view(torch.int64))) <= len(some) * 64
     del keys, out
     torch.cuda.empty_cache()
+
+
+# ---- the range of values ------------------------------------------------------------------------------------------------
+def each_query(t, got, q, n0):
+    """Every query by itself.  A share (weight times its value's scale) is rounded to an f16 (2^-11) and scores are off by 1e-5, together under 2^-10 of every share; the output is a bf16 (2^-8).
+    A query's largest share is 2^5 or more (2^6 times a factor of 1/2 or more when its maximum was taken), and shares under 2^-14 are rounded by 2^-25: by 2^-30 of the largest, each.  (A
+    column where the largest token's number is zero shows that: what the others leave there is small.)"""
+    got = u.host(got).reshape(len(q), t.heads, -1)
+    k, number, ks, vs = t.cache.host()
+    k = k.astype(f64) * ks[..., None]
+    for i in range(len(q)):
+        p = n0 + i
+        first = max(p // t.chunk * t.chunk if t.chunk else 0, p - t.window + 1 if t.window else 0)
+        for h in range(t.heads):
+            kvh = h // (t.heads // t.kv)
+            s = k[kvh, 0, first:p + 1, :t.dim] @ q[i, h].astype(f64)
+            e = np.exp(s - s.max())
+            share, x = e / e.sum() * vs[kvh, first:p + 1], number[kvh, first:p + 1].astype(f64)
+            want = share @ x
+            off = np.abs(got[i, h] - want) - (2.0 ** -8 * np.abs(want) + 2.0 ** -10 * (share @ np.abs(x)) + 2.0 ** -30 * share.max() * np.abs(x).sum(0))
+            assert off.max() <= 0, (p, h, off.argmax(), got[i, h, off.argmax()], want[off.argmax()])
+
+
+def prompted_by_value(hip, t, n0, n):
+    t.convolved = t.rows[:, :t.channels].astype(f64)
+    if n0:
+        t.fill(hip, 0, n0)
+    _, q = t.fill(hip, n0, n)
+    q = as_bf16(q) if t.f32 else q
+    qh = u.host(q).reshape(n - n0, -1, t.dimp)[..., :t.dim]
+    for split in (True, False):
+        each_query(t, t.prompt(hip, q, n0, n, split), qh, n0)
+
+
+@pytest.mark.parametrize("up", [-112, -100, -80, 60, 100])
+@pytest.mark.parametrize("shape", [(4, 2, 64, 64), (4, 1, 128, 128), (2, 1, 200, 200)])
+def test_values_all_small_or_all_large(hip, pkg, shape, up):
+    """down to what a cache's scale can hold"""
+    t = kv.Attention(pkg, 200, *shape, normed=False, f32=True)
+    t.rows[:, t.channels - t.kv * t.vdimp:t.channels] *= np.float32(2.0 ** up)
+    prompted_by_value(hip, t, 0, 200)
+    t.check(t.step(hip, 199), t.want(t.q[199:], 199), STEP)
+
+
+@pytest.mark.parametrize("up", [10, 24, 33, 50])
+@pytest.mark.parametrize("where", ["later", "ahead of the window", "ahead of the chunk"])
+@pytest.mark.parametrize("shape", [(4, 2, 64, 64), (4, 1, 128, 128), (2, 1, 200, 200)])
+def test_a_large_value_that_a_query_does_not_see(hip, pkg, shape, where, up):
+    """in the same tile of keys, and tiles away"""
+    for n0, n in ((0, 250), (100, 330)):
+        options = {"later": {}, "ahead of the window": dict(window=40), "ahead of the chunk": dict(chunk=90)}[where]
+        t = kv.Attention(pkg, n, *shape, normed=False, f32=True, **options)
+        at = t.channels - t.kv * t.vdimp
+        for i, more in ((n0 + 45, 0), (n0 + 140, 8), (n - 1, 9)) if where == "later" else ((3, 0), (70, 3), (n0 + 33, 6), (n0 + 155, 9)):
+            t.rows[i, at:t.channels] *= np.float32(2.0 ** (up + more))
+        prompted_by_value(hip, t, n0, n)
+
+
+@pytest.mark.parametrize("up", [10, 30, 60])
+def test_a_large_value_of_no_weight(hip, pkg, up):
+    """what a query sees and does not weigh leaves the others their bits"""
+    n = 300
+    t = kv.Attention(pkg, n, 4, 2, 64, 64, normed=False, f32=True)
+    nq = 4 * t.dimp
+    t.rows[:, :nq] = np.abs(t.rows[:, :nq])
+    for i in (20, 130, 200):
+        t.rows[i, nq:nq + 2 * t.dimp] = -40.0  # (scores of some -400)
+        t.rows[i, nq + 2 * t.dimp:t.channels] *= np.float32(2.0 ** up)
+    prompted_by_value(hip, t, 0, n)

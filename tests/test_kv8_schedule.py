@@ -16,14 +16,14 @@ int main() {
     const Kv8Schedule kept = bitnet_hip::kKv8Schedule;
     const Kv8Schedule all[] = {
         kept,
-        {{2, 2}, 2, 1, 2, 2},  // keys 32 .. 63 of the tile after next, where those of this tile are read
-        {{1, 1}, 2, 1, 2, 2},  // keys 0 .. 31 of the next tile, where they are read
-        {{2, 1}, 2, 0, 2, 2},  // values of the tile at hand
-        {{2, 1}, 2, 2, 2, 2},  // of the tile after next, over those that are read
-        {{2, 1}, 2, 1, 1, 2},  // factors where they are read
-        {{2, 1}, 2, 1, 3, 2},  // .. and over those that are read
-        {{2, 1}, 2, 1, 2, 1},  // scales and `above` in one place for tiles two apart
-        {{2, 1}, 1, 1, 2, 2},  // scales where they are read
+        {{2, 2}, 2, 1, 1, 2},  // keys 32 .. 63 of the tile after next, where those of this tile are read
+        {{1, 1}, 2, 1, 1, 2},  // keys 0 .. 31 of the next tile, where they are read
+        {{2, 1}, 2, 0, 1, 2},  // values of the tile at hand
+        {{2, 1}, 2, 2, 1, 2},  // of the tile after next, over those that are read
+        {{2, 1}, 2, 1, 0, 2},  // factors where they are read
+        {{2, 1}, 2, 1, 2, 2},  // .. and over those that are read
+        {{2, 1}, 2, 1, 1, 1},  // scales in one place for tiles two apart
+        {{2, 1}, 1, 1, 1, 2},  // scales where they are read
     };
     for (const Kv8Schedule &s : all) std::printf("%d", (int)bitnet_hip::kv8_schedule_holds(s));
 }

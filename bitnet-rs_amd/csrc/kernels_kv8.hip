@@ -56,6 +56,15 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 __device__ __forceinline__ int exponent_above(float v, int least) { return v > 0.f ? max(__builtin_amdgcn_frexp_expf(v), least) : least; }
 __device__ __forceinline__ float power2(int e) { return __builtin_amdgcn_ldexpf(1.0f, e); }
 
+// Shares.  What a value brings to an output is its numbers times a share: its weight, exp2(score - m), times its scale.  Shares meet the numbers in f16, so a scale goes without the power of
+// two that the largest one so far needs (its factor, below 1), and m follows a query's largest share (score plus the factor's exponent) instead of its largest score: whatever else is larger,
+// unseen or without weight, a query's shares lie where f16 holds them.  (A weight alone, of a small value, may be above 1: sums are f32.)  A factor's exponent counts as kBelow at least, which
+// keeps sums finite; and where a larger scale makes all factors smaller by 2^less, m moves down with them as far as the sum has room.
+constexpr int kLeast = -126, kBelow = -64;  // of scales, of factors
+// (of a factor that is held times 2^up)
+__device__ __forceinline__ float factor_exponent(float v, int up) { return (float)max((int)(__builtin_bit_cast(uint32_t, v) >> 23) - 126 - up, kBelow); }
+__device__ __forceinline__ int room_for(float sum, int less) { return sum > 0.f ? min(less, max(100 - __builtin_amdgcn_frexp_expf(sum), 0)) : min(less, 100); }
+
 // How a vector of an 8-bit cache is held: whole numbers -127 .. 127 and one scale.  The scale stays 32 bits wide.  What is smaller than 1.5e-36 throughout counts as zero (its scale would
 // have no full mantissa), and a vector with a value that is not finite has a scale that is not a number, so that whoever sees it gets NaN.
 struct Kv8Scale {
@@ -403,7 +412,7 @@ hipError_t launch_kv8_read(const Kv8 &c, int first, int n, void *keys, void *val
 // One workgroup per (record, kv head and 16 of its query heads), four waves; a wave takes every fourth block of 32 keys by itself, with maximum, sum and output of its own, and
 // the four meet at the end.  S^T = K Q^T on whole numbers: row 4 g + e of score tile t is key 8 g + 4 t + e of the block, so that a lane's weights of both tiles are the eight
 // consecutive keys 8 g .. 8 g + 7 which it needs as an operand of O^T = V^T P^T.
-// A weight times its value's scale is brought to at most 2^14 by a power of two that the wave keeps (o is held times 2^(14 - above)).
+// Shares are at most 2^14 (o is held times 2^(14 - above)), in pairs of f16.
 // Bound by memory behind many keys: 131072 of 32 heads on 8 of 128 columns are 277 MB in 47.6 us (5.8 TB/s; reading alone reaches 6.5).  From 63.5 on: neighbouring records joined where a
 // launch has more of them than the chip holds workgroups, which saves a second preparation of the queries, 53.4; loads past the caches 47.6.  By latency behind few: 200 keys of 20 heads on 5
 // 7.0 us, 2090 of 12 on 3 with two maps of 64 / 128 8.0, 4096 in a window of 16 on 2 of 256 10.5.  A launch is a chain of arguments, position, rows, norms, digits, keys, records: every
@@ -601,7 +610,7 @@ __global__ __launch_bounds__(256, step_held(NK, NV, MAPS)) void k_kv8_step(Kv8St
 #pragma unroll
         for (int v = 0; v < NV; ++v) o[v][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    int above = -100;
+    int above = kLeast;
     auto work = [&](int kb, Block &now, Block &then) __attribute__((always_inline)) {
         const bool more = kb + 128 < k1;
         if (kTwo && more) fetch_keys(then, kb + 128), fetch_values(then, kb + 128);
@@ -652,15 +661,24 @@ __global__ __launch_bounds__(256, step_held(NK, NV, MAPS)) void k_kv8_step(Kv8St
 #pragma unroll
                 for (int e = 0; e < 4; ++e) sv[t][e] = seen(t, e) ? sv[t][e] : 0.f;
         const float largest = fmaxf(fmaxf(fmaxf(sv[0][0], sv[0][1]), fmaxf(sv[0][2], sv[0][3])), fmaxf(fmaxf(sv[1][0], sv[1][1]), fmaxf(sv[1][2], sv[1][3])));
-        const int need = __builtin_amdgcn_readfirstlane(exponent_above(rows_max(largest), -100));
+        const int need = __builtin_amdgcn_readfirstlane(exponent_above(rows_max(largest), kLeast));
         if (need > above) {
-            const float down = power2(max(above - need, -140));
+            const int less = need - above;
+            above = need;
 #pragma unroll
-            for (int j = 0; j < MAPS; ++j)
+            for (int j = 0; j < MAPS; ++j) {
+                const int moved = room_for(rows_sum(l[j]), less);
+                const float down = power2(moved - less);
+                m[j] -= (float)moved, l[j] *= power2(moved);
 #pragma unroll
                 for (int v = 0; v < NV; ++v) o[v][j] *= down;
-            above = need;
+            }
         }
+        f32x4 factor[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) factor[t][e] = __builtin_amdgcn_ldexpf(sv[t][e], 14 - above);
         f16x8 hi[MAPS], lo[MAPS];
 #pragma unroll
         for (int j = 0; j < MAPS; ++j) {
@@ -685,7 +703,11 @@ __global__ __launch_bounds__(256, step_held(NK, NV, MAPS)) void k_kv8_step(Kv8St
                 for (int t = 0; t < 2; ++t)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) s[t][e] = seen(t, e) ? s[t][e] : -INFINITY;
-            float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+            float mx = -INFINITY;  // (of shares)
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) mx = fmaxf(mx, s[t][e] + factor_exponent(factor[t][e], 14));
             mx = fmaxf(m[j], rows_max(mx));
             if (__any(mx > m[j] || mx == -INFINITY)) {
                 if (mx == -INFINITY) mx = 0.f;  // (no score is a number: neither is the sum)
@@ -705,7 +727,7 @@ __global__ __launch_bounds__(256, step_held(NK, NV, MAPS)) void k_kv8_step(Kv8St
             for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int e = 0; e < 4; e += 2) {
-                    const float x = w[t][e] * __builtin_amdgcn_ldexpf(sv[t][e], 14 - above), y = w[t][e + 1] * __builtin_amdgcn_ldexpf(sv[t][e + 1], 14 - above);
+                    const float x = w[t][e] * factor[t][e], y = w[t][e + 1] * factor[t][e + 1];
                     // (an instruction by name: left to itself the compiler rounds the product once for the products and another time for what is left of it)
                     const f16x2 h = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(x, y));
                     hi[j][4 * t + e] = h.x, hi[j][4 * t + e + 1] = h.y;
@@ -808,12 +830,9 @@ hipError_t launch_kv8_step(const Kv8 &c, const GqaStep &a, hipStream_t s) {
 
 // ---- prompt -----------------------------------------------------------------------------------------------------------
 constexpr int kv8_tile_bytes(int nk, int nv, int maps) { return maps * 64 * (nk * 128 + 32) + nv * 16 * (64 * 2 + 32); }
-// A share is a weight, exp2(score - m) times 2^kWeightUp, times its value's factor, the scale without the power of two that the largest scale so far needs.  m follows the exponent of a query's
-// largest share (score plus the factor's exponent, of what the query sees) once that may be kLazy above it: shares are at most 2^14 and a query's largest one is 2^6 or more, so that an f16
-// holds 11 bits of all that are 2^-20 of the largest, whatever lies at positions that the query does not see or weigh.  (A weight alone, of a small value, may be larger: sums are f32.)
-// Factors count as 2^kBelow at least in that, which keeps sums finite: scales down to 2^-64 of the largest one up to the portion's end keep their bits.
+// Weights are exp2(score - m) times 2^kWeightUp, and m follows the largest share once that may be kLazy above it: shares are at most 2^14, and a query's largest is 2^5 or more, so that an f16
+// holds 11 bits of all that are 2^-19 of it.
 constexpr float kWeightUp = 6.0f, kLazy = 8.0f, kLittle = 2.0f;
-constexpr int kLeast = -126, kBelow = -64;
 
 // One workgroup: the rows of W waves, a row being a query of one head; the heads that share keys and values are neighbours among the rows (row r: query r / group, head r % group of
 // the kv head).  A wave holds two slots of 16 rows: both maps of one set of rows, or two sets of the only map.  Key tiles of 64 (every map's) and the values of a tile are staged
@@ -1064,7 +1083,7 @@ __global__ __launch_bounds__(64 * W * G, NV > 8 || NK > 2 ? 1 : 2) void k_kv8_pr
 #pragma unroll
             for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) e[kt][i] = (float)exponent_above(factors(kt)[i], kBelow);
+                for (int i = 0; i < 4; ++i) e[kt][i] = factor_exponent(factors(kt)[i], 0);
 #pragma unroll
             for (int t = 0; t < SLOTS; ++t) {
                 float largest = -INFINITY;
@@ -1073,9 +1092,7 @@ __global__ __launch_bounds__(64 * W * G, NV > 8 || NK > 2 ? 1 : 2) void k_kv8_pr
 #pragma unroll
                     for (int i = 0; i < 4; ++i) largest = fmaxf(largest, fmaf(s[kt][t][i], c2[t], e[kt][i]));
                 largest = rows_max(largest);
-                // m moves with the factors as far as the sum has room, so that a query that does not see what is large keeps its bits; the outputs take the rest
-                const float total = rows_sum(l[t]);
-                const int moved = total > 0.f ? min(less, max(100 - __builtin_amdgcn_frexp_expf(total), 0)) : min(less, 100);
+                const int moved = room_for(rows_sum(l[t]), less);
                 const float from = m[t] - (float)moved, to = largest > from + kLittle ? largest : from, al = __builtin_amdgcn_exp2f(from - to), down = power2(moved - less);
                 m[t] = to;
                 l[t] *= al * power2(moved);

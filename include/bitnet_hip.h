@@ -869,10 +869,12 @@ int bitnet_hip_kv8_rows_dev(const bitnet_hip_gqa *attn, float *k_scale_dev, floa
                             size_t ldq, void *stream);
 /* positions first .. first + n - 1 as bf16 or f32: keys [kv_heads][maps][n][dimp], values [kv_heads][n][vdimp], on 16 bytes (either one NULL: left out) */
 int bitnet_hip_kv8_read_dev(const bitnet_hip_gqa *attn, const float *k_scale_dev, const float *v_scale_dev, size_t first, size_t n, void *keys_dev, void *values_dev, int f32, void *stream);
-/* as gqa_step: the row is appended by the same launch (the attention sees it as the cache holds it), and the records are those that gqa_merge, gqa_out and gqa_project take */
+/* as gqa_step: the row is appended by the same launch (the attention sees it as the cache holds it), and the records are those that gqa_merge, gqa_out and gqa_project
+ * take.  Scales below 2^-64 of the largest one that the step sees lose bits. */
 int bitnet_hip_kv8_step_dev(const bitnet_hip_gqa *attn, float *k_scale_dev, float *v_scale_dev, const float *row_dev, const int32_t *pos_dev, float *scratch_dev, void *stream);
-/* as gqa_prefill_scratch (scratch NULL: the keys stay together; two maps of heads of more than 128 columns want the scratch); q as kv8_rows leaves it, out bf16; up to 2^30 rows (queries times heads).  A weighed value is rounded to 2^-11
- * of itself, or 2^-30 of the query's largest one; scales below 2^-64 of the largest one among the n_ctx positions lose bits, whether a query sees that one or not. */
+/* as gqa_prefill_scratch (scratch NULL: the keys stay together; two maps of heads of more than 128 columns want the scratch); q as kv8_rows leaves it, out bf16; up to 2^30 rows (queries
+ * times heads).  A weighed value is rounded to 2^-11 of itself, or 2^-30 of the query's largest one; scales below 2^-64 of the largest one among the n_ctx positions lose bits, whether a
+ * query sees that one or not. */
 size_t bitnet_hip_kv8_prefill_scratch_bytes(const bitnet_hip_gqa *attn, size_t n_ctx, size_t nq);
 int bitnet_hip_kv8_prefill_dev(const bitnet_hip_gqa *attn, const float *k_scale_dev, const float *v_scale_dev, const uint16_t *q_dev, size_t ldq, size_t n_ctx, size_t nq, uint16_t *out_dev,
                                size_t ldo, float *scratch_dev, size_t scratch_bytes, void *stream);

@@ -544,3 +544,20 @@ def test_a_large_value_of_no_weight(hip, pkg, up):
         t.rows[i, nq:nq + 2 * t.dimp] = -40.0  # (scores of some -400)
         t.rows[i, nq + 2 * t.dimp:t.channels] *= np.float32(2.0 ** up)
     prompted_by_value(hip, t, 0, n)
+
+
+@pytest.mark.parametrize("up", [10, 30, 60])
+@pytest.mark.parametrize("shape", [(4, 2, 64, 64, 1), (4, 1, 64, 128, 2), (2, 1, 200, 200, 1)])
+def test_a_large_value_of_no_weight_in_a_step(hip, pkg, shape, up):
+    """shares of 2^-20 of the largest and more keep the 22 bits of a pair of f16 (2^-24 absolute where the largest is 2^5 at least: 2^-30 of it)"""
+    n = 300
+    t = kv.Attention(pkg, n, *shape, normed=False, f32=True)
+    nq, nk = t.heads * t.maps * t.dimp, t.kv * t.maps * t.dimp
+    t.rows[:, :nq] = np.abs(t.rows[:, :nq])
+    for i in (20, 130, 200, 280):
+        t.rows[i, nq:nq + nk] = np.where(np.arange(nk) % t.dimp < t.dim, -40.0, 0.0)  # (scores of some -400)
+        t.rows[i, nq + nk:t.channels] *= np.float32(2.0 ** up)
+    t.convolved = t.rows[:, :t.channels].astype(f64)
+    t.fill(hip, 0, n - 1)
+    q = t.rows[n - 1:, :nq].astype(f64).reshape(1, -1, t.dimp)[..., :t.dim] * t.keep[2][n - 1].item()
+    t.check(t.step(hip, n - 1), t.want(q, n - 1), STEP)

@@ -561,3 +561,20 @@ def test_a_large_value_of_no_weight_in_a_step(hip, pkg, shape, up):
     t.fill(hip, 0, n - 1)
     q = t.rows[n - 1:, :nq].astype(f64).reshape(1, -1, t.dimp)[..., :t.dim] * t.keep[2][n - 1].item()
     t.check(t.step(hip, n - 1), t.want(q, n - 1), STEP)
+
+
+@pytest.mark.parametrize("shape", [(4, 2, 24, 40, 2), (4, 2, 64, 64, 1), (6, 3, 96, 96, 1), (4, 2, 128, 128, 1), (2, 1, 200, 256, 2), (2, 2, 256, 256, 1)])
+@pytest.mark.parametrize("rot", [0, 8, 24])
+def test_a_step_writes_what_a_portion_of_one_writes(hip, pkg, shape, rot):
+    """bit by bit where a norm's sum is exact (whole numbers) and has no order"""
+    n = 60
+    one, step = (kv.Attention(pkg, n, *shape, f32=True, rot=rot) for _ in range(2))
+    for t in (one, step):
+        nk = (t.heads + t.kv) * t.maps * t.dimp
+        t.rows[:, :nk] = np.rint(t.rows[:, :nk] * 3)
+        t.convolved = t.rows[:, :t.channels].astype(f64)
+    for i in range(n):
+        one.fill(hip, i, i + 1)
+        step.step(hip, i)
+    for name, a, b in zip(("keys", "values", "key scales", "value scales"), one.cache.host(), step.cache.host()):
+        assert np.array_equal(a, b), (name, (a != b).mean())

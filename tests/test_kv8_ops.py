@@ -578,3 +578,33 @@ def test_a_step_writes_what_a_portion_of_one_writes(hip, pkg, shape, rot):
         step.step(hip, i)
     for name, a, b in zip(("keys", "values", "key scales", "value scales"), one.cache.host(), step.cache.host()):
         assert np.array_equal(a, b), (name, (a != b).mean())
+
+
+@pytest.mark.parametrize("options", [dict(), dict(sink=True, gate="heads"), dict(gate="columns", window=700)])
+@pytest.mark.parametrize("shape,n", [((20, 5, 128, 128, 1), 1), ((20, 5, 128, 128, 1), 129), ((20, 5, 128, 128, 1), 512), ((12, 3, 96, 96, 1), 1500), ((128, 128, 32, 32, 1), 640),
+                                     ((128, 128, 32, 32, 1), 1100), ((128, 128, 24, 24, 1), 1500)])
+def test_records_into_the_product_behind_them(hip, pkg, shape, n, options):
+    """a step's records, joined ones and the empty ones behind them too (128 heads: two in one from 513 workgroups on, four from 1025), by gqa_project and, up to four, gqa_out: as by
+    gqa_merge and a product in 64 bits"""
+    t = kv.Attention(pkg, n, *shape, f32=True, **options)
+    if n > 1:
+        t.fill(hip, 0, n - 1)
+    scratch = u.zeros_f32(hip.gqa_scratch_bytes(t.heads, 1, t.vdimp, 1) // 4)
+    scratch.fill_(np.nan)
+    out = t.step(hip, n - 1, scratch=scratch)
+    t.check(out, t.want(t.q[n - 1:], n - 1), STEP)
+    cols, rows = t.heads * t.vdimp, 70
+    first = max(0, n - t.window) if t.window else 0
+    records = (n - 1 - first // 128 * 128) // 128 + 1
+    w = u.rounded(np.random.default_rng(n).standard_normal((rows, cols)) / np.sqrt(cols))
+    row = u.dev_f32(t.rows[n - 1])  # (the gate that step took from a buffer of its own)
+    t.gated(row)
+    pos, want = u.dev(np.array([n - 1], np.int32)), w.astype(f64) @ u.host(out).reshape(-1).astype(f64)
+    product = hip.gqa_project_dev, hip.gqa_out_dev
+    for call, most in zip(product, (hip.gqa_project_records(t.attn, cols), hip.gqa_out_records(t.attn, cols))):
+        assert most >= 4
+        if records > most:
+            continue
+        y = u.zeros_f32(rows)
+        call(t.attn, pos, records, scratch, u.dev_bf16(w), rows, cols, cols, y)
+        assert u.rms_error(u.host(y), want) < 3e-6

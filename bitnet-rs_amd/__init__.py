@@ -691,6 +691,11 @@ class HipLib:
     def kv8_prefill_dev(self, a: "Gqa", k_scale, v_scale, q, ldq: int, n_ctx: int, nq: int, out, ldo: int, scratch=None, scratch_bytes: int = 0, stream: int = 0) -> None:
         self._check(self.c.bitnet_hip_kv8_prefill_dev(C.byref(a), _addr(k_scale), _addr(v_scale), _addr(q), ldq, n_ctx, nq, _addr(out), ldo, _addr(scratch), scratch_bytes, stream))
 
+    def kv8_prefill_last_form(self) -> tuple:
+        form = (C.c_int * 3)()
+        self.c.bitnet_hip_kv8_prefill_last_form(*(C.byref(form, 4 * i) for i in range(3)))
+        return tuple(form)
+
     def delta_step_dev(self, d: "Delta", row, ba, pos, out, stream: int = 0) -> None:
         self._call("delta_step_dev", C.byref(d), _ptr(row), _ptr(ba), _ptr(pos), _ptr(out), _vp(stream))
 

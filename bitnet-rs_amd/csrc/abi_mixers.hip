@@ -284,6 +284,12 @@ int bitnet_hip_kv8_prefill_dev(const bitnet_hip_gqa *a, const float *k_scale, co
     BH_GUARD_END
 }
 
+void bitnet_hip_kv8_prefill_last_form(int *groups, int *waves, int *stretches) {
+    if (groups) *groups = g_last_kv8_form.groups;
+    if (waves) *waves = g_last_kv8_form.waves;
+    if (stretches) *stretches = g_last_kv8_form.parts;
+}
+
 // ---- gated delta rule -------------------------------------------------------------------------------------------------
 int bitnet_hip_delta_supported(size_t dimp, size_t vdimp) { return dimp <= 65536 && vdimp <= 65536 && delta_supported((int)dimp, (int)vdimp) ? 1 : 0; }
 int bitnet_hip_delta_chunked_supported(size_t dimp, size_t vdimp) { return dimp <= 65536 && vdimp <= 65536 && delta_chunked_supported((int)dimp, (int)vdimp) ? 1 : 0; }

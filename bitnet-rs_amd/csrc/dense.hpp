@@ -272,6 +272,10 @@ hipError_t launch_kv8_rows(const Kv8 &c, const void *rows, size_t ld, int rows_f
 hipError_t launch_kv8_read(const Kv8 &c, int first, int n, void *keys, void *values, int f32, hipStream_t s);
 hipError_t launch_kv8_step(const Kv8 &c, const GqaStep &a, hipStream_t s);
 bool kv8_prefill_wants_records(const Gqa &g);  // whatever the lengths
+struct Kv8Form {  // of a prompt's launch: groups of waves that share the rows of a workgroup, waves of a group, stretches of the keys
+    int groups, waves, parts;
+};
+extern thread_local Kv8Form g_last_kv8_form;  // of launch_kv8_prefill's last launch on this thread
 size_t kv8_prefill_floats(const Gqa &g, int n_ctx, int nq);
 hipError_t launch_kv8_prefill(const Kv8 &c, const uint16_t *q, size_t ldq, int n_ctx, int nq, uint16_t *out, size_t ldo, float *records, hipStream_t s);
 bool delta_supported(int dimp, int vdimp);

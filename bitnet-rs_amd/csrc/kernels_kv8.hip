@@ -861,7 +861,7 @@ constexpr float kWeightUp = 6.0f, kLazy = 8.0f, kLittle = 2.0f;
 // and 1 in turn), the factors (32 ..) and their exponents (40).
 // FAR: with a distance penalty, gates per column, or both.
 template <int NK, int NV, int MAPS, bool FAR, int G, int W>
-__global__ __launch_bounds__(64 * W * G, NV > 8 || NK > 2 ? 1 : 2) void k_kv8_prefill(Kv8 c, const uint16_t *Q, size_t ldq, int n_ctx, int nq, uint16_t *out, size_t ldo, int n_qb, float *records) {
+__global__ __launch_bounds__(64 * W * G, NV > 8 || NK > 2 || (NK == 2 && MAPS == 2 && W == 4) ? 1 : 2) void k_kv8_prefill(Kv8 c, const uint16_t *Q, size_t ldq, int n_ctx, int nq, uint16_t *out, size_t ldo, int n_qb, float *records) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     constexpr int SLOTS = 2, QW = 16 * SLOTS / MAPS, KK = 2 * NK, KS = NK * 128 + 32, VS = 64 * 2 + 32, T = 64 * W, KC = NK * 4, KR = T / KC, NKL = (MAPS * 64 + KR - 1) / KR, NVL = (NV * 64 + T - 1) / T;
     constexpr int KB = MAPS * 64 * KS, TILE = kv8_tile_bytes(NK, NV, MAPS), PAD = KB + 128;
@@ -1255,23 +1255,25 @@ __global__ __launch_bounds__(64 * W * G, NV > 8 || NK > 2 ? 1 : 2) void k_kv8_pr
 static bool maps_apart(const Gqa &g) { return g.maps == 2 && (g.dimp > 128 || g.vdimp > 128); }
 bool kv8_prefill_wants_records(const Gqa &g) { return maps_apart(g); }
 
-// Waves that share a tile, groups of them that share the rows, and stretches of the keys.  us of a step of a walk (128 columns; other sizes keep the proportions): four waves 1.72, with two
-// such workgroups on a compute unit 2.4; two groups of four waves 2.44 for two tiles; eight waves (twice the rows) 1.98; heads of more than 128 columns 3.3, one workgroup on a compute unit.
-// A launch lasts as long as its longest walk, or as its share of all of them with what workgroups of unequal length leave idle (an eighth; more where few long ones share a compute
-// unit's time).  Records cost 5 us and their bytes, 0.23 ns for 132 floats.
-// us by this rule, and of the others whole: 20 heads on 5 of 128, prompts of 130 / 600 / 2000 / 4000 12.8 / 23.1 / 49.5 / 125 (eight waves 15.4 / 28.6 / 72 / 134, two groups 14.9 / 23.1 / 49.5
-// / 135); 32 on 8, 4000 153 (four waves 176, two groups 195); 509 behind 20011, 12 of two maps, eight waves in 5 stretches 141 (whole 356 and more), 30 behind 7970, 20 heads, 28 (153).
-struct Kv8Form {
-    int groups, waves, parts;
-};
+// Waves that share a tile, groups of them that share the rows, and stretches of the keys.  us of a step of a walk (128 columns): four waves 1.72, with two such workgroups on a compute unit
+// 2.4; two groups of four waves 2.44 for two tiles; eight waves (twice the rows) 1.98; heads of more than 128 columns 3.3, one workgroup on a compute unit; two maps of 65 to 128 columns 2.4
+// whatever the waves, one workgroup.  A launch lasts as long as its longest walk, or as its share of all of them with what workgroups of unequal length leave idle (an eighth; more where few
+// long ones share a compute unit's time).  Records cost 5 us and their bytes, 0.23 ns for 132 floats.
+// Heads of up to 64 columns go by the same figures: they take three quarters of the time in every form.
+// us, what this rule takes / four waves / two groups / eight waves, and in stretches where that is best:
+//   20 heads on 5 of 128: 130 tokens 13 / 13 / 14 / 16; 600 23 / 26 / 23 / 30; 2000 53 / 70 / 53 / 78; 4000 130 / 130 / 141 / 149; 8192 428 / 407 / 459 / 428; 30 behind 7970 28 (157 whole)
+//   32 on 8 of 128: 4000 174 / 186 / 208 / 174; 8192 610 / 626 / 709 / 609; 509 behind 20011 232 (384 whole, 214 in four)
+//   20 on 5 of 64: 4000 101 / 101 / 106 / 116; 8192 338 / 306 / 355 / 335.  8 on 8 of 64: 4000 78 / 95 / 68 / 111 (65); 8192 147 / 189 / 145 / 222
+//   two maps, 12 on 3 of 64 / 128: 4000 131 / 128 / 152 / 139; 509 behind 20011 177 (367 whole).  12 on 3 of 128: 600 32 / 32 / - / 33; 2000 88 / 88 / - / 86 (73); 4000 167 / 273 / - / 167
+thread_local Kv8Form g_last_kv8_form{0, 0, 0};
 static Kv8Form prefill_form(const Gqa &g, int n_ctx, int nq, bool room) {
     const int group = (int)(g.heads / g.kv_heads), maps = maps_apart(g) ? 1 : (int)g.maps, longest = n_ctx / 64 + 1 - (gqa_first(g, n_ctx - 1) >> 6);
     const double shortest = (n_ctx - nq) / 64 + 1 - (gqa_first(g, n_ctx - nq) >> 6), record = 0.23e-3 * (kGqaRecHead + g.vdimp) / 132 * nq * g.heads * g.maps;
-    const bool wide = g.dimp > 128 || g.vdimp > 128;
+    const bool wide = g.dimp > 128 || g.vdimp > 128, both = maps == 2 && g.dimp > 64;  // (keys of both maps: LDS has room for one workgroup)
     Kv8Form best{1, 4, 1};
     double least = 1e30;
     for (const Kv8Form f : {Kv8Form{1, 4, 1}, Kv8Form{2, 4, 1}, Kv8Form{1, 8, 1}}) {
-        if ((wide && (f.groups == 2 || f.waves == 8)) || (f.groups == 2 && maps == 2 && g.dimp > 64)) continue;
+        if ((wide && (f.groups == 2 || f.waves == 8)) || (f.groups == 2 && both)) continue;
         const int rows = 32 * f.waves / maps;
         const double workgroups = (double)g.kv_heads * ((nq * (size_t)group + rows - 1) / rows) * (maps_apart(g) ? 2 : 1);
         for (int parts = 1; parts <= (room ? 32 : 1) && (parts == 1 || (2 * parts <= longest && workgroups * parts <= 512)); ++parts) {
@@ -1280,6 +1282,8 @@ static Kv8Form prefill_form(const Gqa &g, int n_ctx, int nq, bool room) {
             double us;
             if (wide)
                 us = 3.3 * std::max(walk, 1.12 * all / 256);
+            else if (both)
+                us = (f.waves == 8 ? 2.5 : 0.0) + 2.4 * std::max(walk, 1.12 * all / 256);
             else if (f.groups == 2)
                 us = 2.0 + 2.44 * std::max(walk, 1.4 * all / 256);
             else if (f.waves == 8)
@@ -1320,7 +1324,7 @@ static hipError_t prefill_go(const Kv8 &c, const uint16_t *q, size_t ldq, int n_
 
 template <int NK, int NV>
 static hipError_t prefill_pick(const Kv8 &c, const uint16_t *q, size_t ldq, int n_ctx, int nq, uint16_t *out, size_t ldo, float *records, hipStream_t s) {
-    const Kv8Form f = prefill_form(c.g, n_ctx, nq, records != nullptr);
+    const Kv8Form f = g_last_kv8_form = prefill_form(c.g, n_ctx, nq, records != nullptr);
     if constexpr (NV <= 8) {
         if (f.groups == 2) return prefill_go<NK, NV, 2, 4>(c, q, ldq, n_ctx, nq, out, ldo, records, f.parts, s);
         if (f.waves == 8) return prefill_go<NK, NV, 1, 8>(c, q, ldq, n_ctx, nq, out, ldo, records, f.parts, s);

@@ -878,6 +878,8 @@ int bitnet_hip_kv8_step_dev(const bitnet_hip_gqa *attn, float *k_scale_dev, floa
 size_t bitnet_hip_kv8_prefill_scratch_bytes(const bitnet_hip_gqa *attn, size_t n_ctx, size_t nq);
 int bitnet_hip_kv8_prefill_dev(const bitnet_hip_gqa *attn, const float *k_scale_dev, const float *v_scale_dev, const uint16_t *q_dev, size_t ldq, size_t n_ctx, size_t nq, uint16_t *out_dev,
                                size_t ldo, float *scratch_dev, size_t scratch_bytes, void *stream);
+/* How the calling thread's last launch of it was shared out (0: none yet): groups of waves that share the rows of a workgroup, waves of a group, stretches of the keys.  Any may be NULL. */
+void bitnet_hip_kv8_prefill_last_form(int *groups, int *waves, int *stretches);
 
 /* Gated delta rule.  A row of projections is [q kv_heads * dimp | k kv_heads * dimp | v heads * vdimp | gate heads * vdimp], and apart from it
  * [b heads | a heads] f32; heads zero-padded to multiples of 32.  q, k, v pass a causal convolution of `taps` tokens per channel and

@@ -486,7 +486,7 @@ def each_query(t, got, q, n0):
     k, number, ks, vs = t.cache.host()
     k = k.astype(f64) * ks[..., None]
     for i in range(len(q)):
-        p = n0 + i
+        p = n0 + i if np.ndim(n0) == 0 else n0[i]
         first = max(p // t.chunk * t.chunk if t.chunk else 0, p - t.window + 1 if t.window else 0)
         for h in range(t.heads):
             kvh = h // (t.heads // t.kv)
@@ -608,3 +608,60 @@ def test_records_into_the_product_behind_them(hip, pkg, shape, n, options):
         y = u.zeros_f32(rows)
         call(t.attn, pos, records, scratch, u.dev_bf16(w), rows, cols, cols, y)
         assert u.rms_error(u.host(y), want) < 3e-6
+
+
+# ---- every form of a prompt's launch --------------------------------------------------------------------------------------
+# columns (keys, values), maps | groups, waves, stretches or not: heads, kv heads, keys, queries
+FORMS = {
+    (24, 64, 1): {(1, 4, False): (3, 1, 130, 130), (1, 4, True): (3, 1, 333, 111), (2, 4, False): (3, 1, 333, 111), (2, 4, True): (3, 1, 2000, 2000), (1, 8, False): (100, 5, 1000, 1000),
+                  (1, 8, True): (6, 1, 2000, 2000)},
+    (64, 100, 1): {(1, 4, False): (3, 1, 130, 130), (1, 4, True): (3, 1, 333, 111), (2, 4, False): (3, 1, 333, 111), (2, 4, True): (3, 1, 1600, 1600), (1, 8, False): (100, 5, 1000, 1000),
+                   (1, 8, True): (32, 4, 2000, 500)},
+    (100, 128, 1): {(1, 4, False): (3, 1, 130, 130), (1, 4, True): (3, 1, 333, 111), (2, 4, False): (3, 1, 333, 111), (2, 4, True): (3, 1, 1600, 1600), (1, 8, False): (100, 5, 1000, 1000),
+                    (1, 8, True): (32, 4, 2000, 500)},
+    (200, 256, 1): {(1, 4, False): (3, 1, 333, 111), (1, 4, True): (3, 1, 333, 111)},
+    (24, 64, 2): {(1, 4, False): (3, 1, 130, 130), (1, 4, True): (1, 1, 333, 333), (2, 4, False): (1, 1, 333, 333), (2, 4, True): (2, 1, 1600, 1600), (1, 8, False): (100, 5, 500, 500),
+                  (1, 8, True): (3, 1, 2000, 2000)},
+    (64, 100, 2): {(1, 4, False): (3, 1, 130, 130), (1, 4, True): (1, 1, 333, 333), (2, 4, False): (1, 1, 333, 333), (2, 4, True): (2, 1, 1600, 1600), (1, 8, False): (100, 5, 500, 500),
+                   (1, 8, True): (16, 4, 2000, 500)},
+    (100, 128, 2): {(1, 4, False): (3, 1, 130, 130), (1, 4, True): (1, 1, 333, 333), (1, 8, False): (60, 3, 500, 500), (1, 8, True): (3, 1, 1600, 1600)},
+    (200, 160, 2): {(1, 4, False): (3, 1, 60, 60), (1, 4, True): (3, 1, 333, 111)},
+}
+FORM_CASES = [(columns, form, shape, options) for columns, forms in FORMS.items() for form, shape in forms.items()
+              for options in ([dict(rot=8)] if columns[2] == 2 else [dict(rot=8), dict(far=True), dict(gate="columns", sink=True), dict(far=True, gate="columns", rot=24)])]
+
+
+@pytest.mark.parametrize("columns,form,shape,options", FORM_CASES)
+def test_every_form_of_a_prompt(hip, pkg, columns, form, shape, options):
+    """each way in which a launch can be shared out, with and without what stands in the instances of its own (penalty, gates by columns); a sample of the queries by definition"""
+    heads, kvh, n, nq = shape
+    t = kv.Attention(pkg, n, heads, kvh, *columns, fill=-128, scale=np.nan, **options)
+    if n > nq:
+        t.fill(hip, 0, n - nq)
+    rows, q = t.fill(hip, n - nq, n)
+    out = t.prompt(hip, q, n - nq, n, split=form[2])
+    groups, waves, stretches = hip.kv8_prefill_last_form()
+    assert (groups, waves, stretches > 1) == form
+    some = np.unique(np.concatenate([np.linspace(0, nq - 1, 9).astype(int), [min(nq - 1, 31), min(nq - 1, 64), nq - 2]]))
+    held, qh = t.cache.held(), u.host(q).reshape(nq, -1, t.dimp)[..., :t.dim]
+    want = np.concatenate([t.want(qh[i:i + 1], n - nq + i, held) for i in some])
+    t.check(u.dev_f32(u.host(out)[some]), want, *PROMPT)
+
+
+@pytest.mark.parametrize("columns,form,shape", [(columns, form, shape) for columns, forms in FORMS.items() if columns[2] == 1 for form, shape in forms.items()])
+def test_every_form_beside_large_values(hip, pkg, columns, form, shape):
+    """large values that the queries ahead of them do not see, in every stretch and group"""
+    heads, kvh, n, nq = shape
+    t = kv.Attention(pkg, n, heads, kvh, *columns, normed=False, f32=True)
+    first = t.channels - t.kv * t.vdimp
+    for i, up in zip(np.linspace(n - nq, n - 1, 7).astype(int), (0, 20, 26, 31, 37, 41, 60)):
+        t.rows[i, first:t.channels] *= np.float32(2.0 ** up)
+    if n > nq:
+        t.fill(hip, 0, n - nq)
+    _, q = t.fill(hip, n - nq, n)
+    q = as_bf16(q)
+    out = t.prompt(hip, q, n - nq, n, split=form[2])
+    groups, waves, stretches = hip.kv8_prefill_last_form()
+    assert (groups, waves, stretches > 1) == form
+    some = np.unique(np.concatenate([np.linspace(0, nq - 2, 9).astype(int), np.linspace(0, nq - 1, 7).astype(int)[1:] - 1]))
+    each_query(t, u.dev_f32(u.host(out)[some]), u.host(q).reshape(nq, -1, t.dimp)[some][..., :t.dim], n - nq + some)

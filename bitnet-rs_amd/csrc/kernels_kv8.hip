@@ -338,13 +338,16 @@ static hipError_t rows_launch(const Kv8 &c, const void *rows, size_t ld, const i
     const bool few = n <= at_once;  // (a wave takes its tokens at once, else four times as many in turn)
     const int each = few ? at_once : 4 * at_once, blocks = (n + each - 1) / each;
     const int chunks = std::min(heads, std::max({1, (heads + 7) / 8, 1280 / blocks}));  // (of heads: all of them where the tokens alone fill the chip, up to eight by a wave in turn)
-    // values: a wave takes 32 positions where that fills the chip (16384 tokens 70.4 us with the read behind, 71.3 by eights), else eight (1531 tokens 7.0, 9.1 by 32)
+    // values: a wave takes 32 positions where that fills the chip (us of 16384 tokens, by 32 / by eights: 8 heads on 8 of 64 20.9 / 24.3, 12 on 3 of 64 18.6 / 18.1, 20 on 5 of 128 42.5 / 41.7;
+    // 1531 tokens of two maps 9.1 / 7.0), else eight
     auto groups = [&](int vp) { return g.queries_only ? 0 : ((n + 2 * vp - 2) / vp + 3) / 4 * (int)g.kv_heads; };  // (n tokens reach into (n + 2 vp - 2) / vp such pieces at most)
     const bool many = !few && groups(32) >= 512;
-    auto fn = few ? k_kv8_rows<TR, KL, VL, TAPS, 1, 8> : many ? k_kv8_rows<TR, KL, VL, TAPS, 4, 32> : k_kv8_rows<TR, KL, VL, TAPS, 4, 8>;
+    // three taps: unrolled for few tokens (us of one, unrolled / looped: 20 heads on 5 of 128 4.3 / 4.7, 16 on 2 of 256 5.2 / 6.0), looped for more (1531: 21 / 16, 27 / 21; 16384: 179 / 145, 276 / 240)
+    auto fn = few ? (TAPS < 0 && g.taps == 3 ? k_kv8_rows<TR, KL, VL, TAPS < 0 ? 3 : TAPS, 1, 8> : k_kv8_rows<TR, KL, VL, TAPS, 1, 8>) : many ? k_kv8_rows<TR, KL, VL, TAPS, 4, 32> : k_kv8_rows<TR, KL, VL, TAPS, 4, 8>;
     hipLaunchKernelGGL(fn, dim3((size_t)blocks * chunks + groups(many ? 32 : 8)), dim3(256), 0, s, c, (const TR *)rows, ld, pos, n, (TR *)q, ldq, blocks, chunks);
     return hipGetLastError();
 }
+// Lanes of a row by its columns (us of 16384 tokens, this / as for wider heads: 64 columns 20.9 / 25.1 with sixteen lanes for the values and 30.7 for both; 64 / 128 of two maps 26.9 / 37.6)
 template <class TR, int TAPS>
 static hipError_t rows_go(const Kv8 &c, const void *rows, size_t ld, const int *pos, int n, void *q, size_t ldq, hipStream_t s) {
     if (c.g.dimp > 128 || c.g.vdimp > 128) return rows_launch<TR, 32, 32, TAPS>(c, rows, ld, pos, n, q, ldq, s);
@@ -353,7 +356,7 @@ static hipError_t rows_go(const Kv8 &c, const void *rows, size_t ld, const int *
 }
 template <class TR>
 static hipError_t rows_taps(const Kv8 &c, const void *rows, size_t ld, const int *pos, int n, void *q, size_t ldq, hipStream_t s) {
-    return c.g.taps == 0 ? rows_go<TR, 0>(c, rows, ld, pos, n, q, ldq, s) : c.g.taps == 3 ? rows_go<TR, 3>(c, rows, ld, pos, n, q, ldq, s) : rows_go<TR, -1>(c, rows, ld, pos, n, q, ldq, s);
+    return c.g.taps == 0 ? rows_go<TR, 0>(c, rows, ld, pos, n, q, ldq, s) : rows_go<TR, -1>(c, rows, ld, pos, n, q, ldq, s);
 }
 hipError_t launch_kv8_rows(const Kv8 &c, const void *rows, size_t ld, int rows_f32, const int *pos, int n, void *q, size_t ldq, hipStream_t s) {
     return rows_f32 ? rows_taps<float>(c, rows, ld, pos, n, q, ldq, s) : rows_taps<uint16_t>(c, rows, ld, pos, n, q, ldq, s);

@@ -665,3 +665,28 @@ def test_every_form_beside_large_values(hip, pkg, columns, form, shape):
     assert (groups, waves, stretches > 1) == form
     some = np.unique(np.concatenate([np.linspace(0, nq - 2, 9).astype(int), np.linspace(0, nq - 1, 7).astype(int)[1:] - 1]))
     each_query(t, u.dev_f32(u.host(out)[some]), u.host(q).reshape(nq, -1, t.dimp)[some][..., :t.dim], n - nq + some)
+
+
+@pytest.mark.parametrize("f32", [True, False])
+@pytest.mark.parametrize("shape,n0,n", [((64, 64, 32, 32, 1), 5, 1100), ((30, 30, 24, 40, 2), 32, 2300)])
+def test_many_tokens_of_many_heads_of_either_type(hip, pkg, shape, n0, n, f32):
+    """values by pieces of 32 positions, as test_many_tokens_of_many_heads"""
+    test_written_bit_by_bit(hip, pkg, shape, n0, n, f32)
+
+
+@pytest.mark.parametrize("f32", [True, False])
+@pytest.mark.parametrize("taps", [1, 3, 5])
+@pytest.mark.parametrize("shape,n0,n", [((40, 40, 64, 64, 1), 13, 1700), ((32, 32, 24, 40, 2), 45, 2100), ((16, 16, 100, 128, 1), 70, 4200), ((6, 2, 200, 256, 1), 33, 300)])
+def test_convolutions_of_many_tokens(hip, pkg, shape, n0, n, taps, f32):
+    """pieces of 32 positions and of eight; a second portion that begins inside a tile, with the first one's last rows in the ring"""
+    t = kv.Attention(pkg, n0 + n, *shape, f32=f32, taps=taps)
+    for a, b in ((0, n0), (n0, n0 + n)):
+        _, q = t.fill(hip, a, b)
+        got = u.host(q).reshape(b - a, -1, t.dimp)
+        assert u.rms_error(got[..., :t.dim], t.q[a:b]) < (3e-6 if f32 else 2.0 ** -8)
+    k, v, ks, vs = t.cache.host()
+    for got, scales, x in ((k, ks, t.k), (v, vs, t.v)):
+        got, scales = got[..., :n0 + n, :].astype(np.float32), scales[..., :n0 + n]
+        largest = np.abs(x).max(-1)
+        assert np.abs(scales * 127 / largest - 1).max() < 1e-5
+        assert (np.abs(got * scales[..., None] - x) <= scales[..., None] * 0.5 + 1e-5 * largest[..., None]).all()

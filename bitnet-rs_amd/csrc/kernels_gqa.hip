@@ -15,6 +15,28 @@
 
 namespace bitnet_hip {
 
+// The records of a query at `pos`: tiles of keys from `base` (the tile that holds its first key) on, `per` tiles each.
+struct GqaRange {
+    int first, base, per, used;
+};
+__device__ __forceinline__ GqaRange gqa_range(const Gqa &p, int pos) {
+    GqaRange r;
+    r.first = gqa_first(p, pos);
+    r.base = r.first & ~(kGqaTile - 1);
+    const int tiles = (pos + 1 - r.base + kGqaTile - 1) / kGqaTile;
+    r.per = (tiles + kGqaSplits - 1) / kGqaSplits;
+    r.used = (tiles + r.per - 1) / r.per;
+    return r;
+}
+
+// element i of a head at a position, v being its own and the lane's neighbour holding the other element of the pair; cs, sn: the tables' row
+__device__ __forceinline__ float turn_neighbours(float v, int i, const float *cs, const float *sn, int dims) {
+    const float o = dpp<0xb1>(v);  // quad_perm [1,0,3,2]
+    if (i >= dims) return v;
+    const float c = cs[i >> 1], s = sn[i >> 1];
+    return (i & 1) ? v * c + o * s : v * c - o * s;
+}
+
 size_t gqa_scratch_floats(size_t heads, size_t maps, size_t vdimp, size_t nq) { return nq * heads * maps * kGqaSplits * (kGqaRecHead + vdimp); }
 bool gqa_supported(int dimp, int vdimp) { return dimp <= 256 && vdimp <= 256; }
 
@@ -1169,6 +1191,23 @@ __global__ __launch_bounds__(256 * G, NV > 8 || NK > 4 ? 1 : 2) void k_gqa_prefi
 
 thread_local int g_last_gqa_groups;
 
+// Two groups fill a CU, and halve its walks; of one group two workgroups fit.  They pay while the launch is as long as its longest walk: with four tiles or more in it, a CU's
+// share of all tiles not much above it, and no second round behind walks that are all long (the shortest walk of the first round and the longest of the second one in turn).
+// Heads count as a multiple of eight, as the launch deals them to the XCDs (20 heads take what 24 do).  us with two / with one: 24 heads, 2600 tokens
+// 80 / 90 (share / walk 1.05), 32 heads, 2048 63 / 75 (1.06), 40 heads, 1664 63 / 62 (1.09), 24 heads, 3000 105 / 105 (1.19), 3328 124 / 121 (1.27), 4096 173 / 153 (1.55); two maps,
+// 24 heads, 1280 39 / 44, 1531 57 / 53, 2048 88 / 75; five tiles 13.1 / 13.9, four 13.0 / 12.4.
+static bool two_groups(const Gqa &g, int rows, int n_ctx, int nq) {
+    const int at_once = 256, pos0 = n_ctx - nq, heads = ((int)g.heads + 7) / 8 * 8, blocks = (nq + rows - 1) / rows, all_tiles = (n_ctx + 63) / 64;
+    long longest = 0, total = 0, second = 0;
+    for (int qb = blocks - 1, done = 0; qb >= 0 && total <= 2l * at_once * all_tiles; --qb, done += heads) {
+        const int q0 = qb * rows, tiles = (std::min(n_ctx, pos0 + q0 + rows) + 63) / 64 - (gqa_first(g, pos0 + q0) >> 6);
+        longest = std::max<long>(longest, tiles), total += (long)heads * tiles;
+        for (int i : {at_once - 1, at_once})
+            if ((long)heads * blocks > at_once && done <= i && i < done + heads) second += tiles;
+    }
+    return longest >= 4 && 16 * total <= 17 * at_once * longest && 10 * second <= 11 * longest;
+}
+
 // The records of a query's head (gridDim.y of the launch above, one behind the other for every map) -> its output: a wave each, vdimp / 4 lanes of four columns, as many groups of them as fit a wave
 // sharing the records.
 template <int MAPS>
@@ -1212,6 +1251,19 @@ __global__ __launch_bounds__(256) void k_gqa_merge_parts(Gqa p, const float *rec
     if (grp == 0) *reinterpret_cast<bf16x4 *>(out + (size_t)qi * ldo + (size_t)h * vdimp + c) = bf16x4{(__bf16)q.x, (__bf16)q.y, (__bf16)q.z, (__bf16)q.w};
 }
 
+// Few queries behind many keys: a launch whose blocks leave CUs without a workgroup lasts as long as its longest walk, so a block's tiles are cut into stretches, of two tiles (a step of two
+// groups) at least and no more of them than there are CUs for (heads count as a multiple of eight, as the launch deals them to the XCDs: 12 heads in 21 stretches take 32 us where 15 take 24).
+// A step of a walk that is saved is worth 2.7 us (7 of one group); the launch that puts the records together costs 5 and 0.7 ns for each query's head, 1.4 for each of a head's two maps.
+// us without / with, heads, keys, queries: 12, 2090, 90 51 / 18; 24, 2090, 90 52 / 22; 12, 600, 20 18.3 / 11.1; 12, 1000, 200 28.7 / 18.9; 12, 450, 130 17.7 / 14.5; 12, 8000, 30 168 / 27;
+// 24 of two maps, 2090, 90 49 / 28; 2 of 256 columns, 2000, 50 131 / 22; 8, 2000, 2000 50 / 40.  What stays whole: 12, 400, 400 15.9 / 18.1; 16, 512, 512 18.6 / 21.2; 24 of two maps,
+// 600, 100 18.3 / 20.6; 12, 100, 3 8.4.
+static int gqa_prefill_parts(const Gqa &g, int n_ctx, int nq) {
+    const int rows = g.maps == 2 ? 64 : 128, blocks = (nq + rows - 1) / rows, heads = ((int)g.heads + 7) / 8 * 8;
+    const int tiles = (n_ctx + 63) / 64 - (gqa_first(g, n_ctx - nq + (blocks - 1) * rows) >> 6), most = std::min<long>(256 / ((long)heads * blocks), 32);
+    if (most < 2) return 1;
+    const int each = ((tiles + most - 1) / most + 1) & ~1, saved = (tiles + 1) / 2 - each / 2;
+    return 2.7 * saved > 5.0 + (g.maps == 2 ? 1.4e-3 : 7e-4) * (double)nq * (double)(g.heads * g.maps) ? (tiles + each - 1) / each : 1;
+}
 hipError_t launch_gqa_merge_parts(const Gqa &g, const float *records, int parts, int nq, uint16_t *out, size_t ldo, hipStream_t s) {
     hipLaunchKernelGGL(g.maps == 2 ? k_gqa_merge_parts<2> : k_gqa_merge_parts<1>, dim3((nq * (int)g.heads + 3) / 4), dim3(256), 0, s, g, records, parts, nq, out, ldo);
     return hipGetLastError();

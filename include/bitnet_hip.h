@@ -863,7 +863,8 @@ int bitnet_hip_gqa_prefill_last_groups(void);
  * outputs that weigh it are none either.  In the attention's description kcache is int8 [kv_heads][maps][capacity][dimp], vcache int8 [kv_heads][capacity / 32][vdimp / 32][16][4][2][8]:
  * column c at position p in [p / 32][c / 32][c % 16][p % 32 / 8][c % 32 / 16][p % 8].  k_scale [kv_heads][maps][capacity], v_scale [kv_heads][capacity].  All four on 16 bytes; nothing has to
  * be cleared first (what lies past the positions written is not used).  The cache is a function of the tokens: portions of any sizes write the same bytes, a step those of a portion of one
- * but for the order of a norm's sum.  Every position can be written again.  Heads of up to 256 columns (bitnet_hip_gqa_supported; others are refused). */
+ * but for the order of a norm's sum.  Every position can be written again.  Scores are right for queries (norm, rotation and factor behind them) of 2^-99 and more and keys
+ * below 2^100, by their largest magnitudes: smaller queries lose bits or count as zero, scores of larger keys may be none.  Heads of up to 256 columns (bitnet_hip_gqa_supported; others are refused). */
 /* as gqa_rows; rows and queries on 16 bytes and, for several tokens, multiples of 8 elements apart; the convolution's taps on 16 bytes */
 int bitnet_hip_kv8_rows_dev(const bitnet_hip_gqa *attn, float *k_scale_dev, float *v_scale_dev, void *rows_dev, size_t ld, int rows_f32, const int32_t *pos_dev, size_t n, void *q_dev,
                             size_t ldq, void *stream);

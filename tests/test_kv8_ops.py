@@ -690,3 +690,9 @@ def test_convolutions_of_many_tokens(hip, pkg, shape, n0, n, taps, f32):
         largest = np.abs(x).max(-1)
         assert np.abs(scales * 127 / largest - 1).max() < 1e-5
         assert (np.abs(got * scales[..., None] - x) <= scales[..., None] * 0.5 + 1e-5 * largest[..., None]).all()
+
+
+@pytest.mark.parametrize("up", [95, -95])
+def test_queries_and_keys_at_the_ends_of_their_range(hip, pkg, up):
+    """queries of some 2^-98 and keys of some 2^98, and the other way round"""
+    test_queries_and_keys_of_opposite_size(hip, pkg, up)

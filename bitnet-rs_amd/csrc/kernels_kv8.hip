@@ -93,8 +93,8 @@ __device__ __forceinline__ size_t kv8_value_at(int vdimp, int pos, int c) {
 }
 
 // ---- rows of projections ----------------------------------------------------------------------------------------------
-// Bound by memory: 16384 tokens of 20 heads on 5 of 128 columns, bf16, half of them turned, are 232 MB in 52 us (4.5 TB/s; a copy reaches 5.3).  By heads first and pairs of columns it
-// was 80, whole rows at a time 64; a wave's heads in turn, with the rotation and the next columns in registers, took the rest.  One token 3.8, 1531 of two maps of 64 / 128 7.0.
+// Bound by memory: 16384 tokens of 20 heads on 5 of 128 columns, bf16, half of them turned, are 232 MB in 53 us (4.4 TB/s; a copy reaches 5.3 to 5.5).  By heads first and pairs of columns it
+// was 80, whole rows at a time 64; a wave's heads in turn, with the rotation and the next columns in registers, took the rest.  One token 3.7, 1531 of two maps of 64 / 128 7.2.
 // A lane holds eight neighbouring columns, KL or VL lanes a head's row: pairs turn within a lane, and a wave takes 64 / KL tokens at a time, R times.  Workgroups: four waves'
 // tokens and a part of the heads (query heads x maps, key heads x maps; one after the other, the next one's columns on their way), then values, eight or 32
 // positions a wave, through LDS into the cache's order.
@@ -364,7 +364,7 @@ hipError_t launch_kv8_rows(const Kv8 &c, const void *rows, size_t ld, int rows_f
 
 // ---- positions read back ----------------------------------------------------------------------------------------------
 // blockIdx.y: key heads x maps (16 bytes a thread), then value heads (a tile of 32 positions a workgroup, turned round in LDS).
-// Bound by memory: 131072 positions of 8 heads of 128 columns as bf16 are 814 MB in 148 us (5.5 TB/s, what a copy reaches); 300 of 3 heads of 80 as f32 3.0.
+// Bound by memory: 131072 positions of 8 heads of 128 columns as bf16 are 814 MB in 148 us (5.5 TB/s; a copy of as much 5.3, writing alone 6.9); 300 of 3 heads of 80 as f32 3.0.
 template <class TO>
 __device__ __forceinline__ void store_numbers(TO *dst, uint32_t numbers, float scale) {  // four of them
     f32x4 v;
@@ -425,8 +425,8 @@ hipError_t launch_kv8_read(const Kv8 &c, int first, int n, void *keys, void *val
 // the four meet at the end.  S^T = K Q^T on whole numbers: row 4 g + e of score tile t is key 8 g + 4 t + e of the block, so that a lane's weights of both tiles are the eight
 // consecutive keys 8 g .. 8 g + 7 which it needs as an operand of O^T = V^T P^T.
 // Shares are at most 2^14 (o is held times 2^(14 - above)), in pairs of f16.
-// Bound by memory behind many keys: 131072 of 32 heads on 8 of 128 columns are 277 MB in 47.6 us (5.8 TB/s; reading alone reaches 6.5).  From 63.5 on: neighbouring records joined where a
-// launch has more of them than the chip holds workgroups, which saves a second preparation of the queries, 53.4; loads past the caches 47.6.  By latency behind few: 200 keys of 20 heads on 5
+// Bound by memory behind many keys: 131072 of 32 heads on 8 of 128 columns are 277 MB in 49 us (5.7 TB/s; reading alone reaches 7.0).  From 63.5 on: neighbouring records joined where a
+// launch has more of them than the chip holds workgroups, which saves a second preparation of the queries, 53.4; loads past the caches 47.6 (shares instead of weights under the maximum 1 more).  By latency behind few: 200 keys of 20 heads on 5
 // 7.0 us, 2090 of 12 on 3 with two maps of 64 / 128 8.0, 4096 in a window of 16 on 2 of 256 10.5.  A launch is a chain of arguments, position, rows, norms, digits, keys, records: every
 // argument is asked for at once and what does not hang on the position ahead of it (7.5, 8.2 and 11.6 without).
 struct Kv8StepK {
@@ -851,12 +851,12 @@ constexpr float kWeightUp = 6.0f, kLazy = 8.0f, kLittle = 2.0f;
 // through registers into LDS.  G = 2: two such groups of W waves share the keys of the same rows, tile by tile in turn, and meet in LDS at the end.  records: gridDim.y workgroups
 // share a block's tiles of keys, in stretches (launch_gqa_merge_parts).  MAPS = 1 with two maps, whose keys together find no room in LDS: gridDim.z is the map, with records.
 // In LDS keys are their numbers + 1152 as f16 (exact; a row's sum times 1152 is what its scores start from), and so is a query of bf16 times a power of two: scores are exact but
-// for the f32 sums, a key's scale meets them in f32.  Values are their numbers (exact in f16), and a weight times its value's factor is rounded to f16 once, to the nearest
+// for the f32 sums (partial sums up to ten times the size that the numbers alone would have, 2^-20 of it together), a key's scale meets them in f32.  Values are their numbers (exact in f16), and a weight times its value's factor is rounded to f16 once, to the nearest
 // (2^-11 of it at most, 1.5e-4 of an output that is rounded to 2^-8 afterwards; f16 pairs would double these products).
 // The products of a SIMD's two waves and their vector instructions take about the same time, and as phases of their own they add up: hence the next tile's scores are made among
 // this tile's exponentials, and this tile's outputs among the staging of the tiles to come.
-// Bound by both pipes of a SIMD: 8192 tokens of 20 heads on 5 of 128 columns, 344 GFLOP, take 420 us (0.82 PFLOP/s, a large product of f16 reaches 1.35; over a cache of bf16 k_gqa_prefill
-// takes 522); 509 tokens behind 20011 of 12 heads on 3 with two maps of 64 / 128 148 us (0.64), 130 tokens of 12 heads 12.6.  Phases one behind the other, two groups of four waves: 515,
+// Bound by both pipes of a SIMD: 8192 tokens of 20 heads on 5 of 128 columns, 344 GFLOP, take 422 us (0.82 PFLOP/s, a large product of f16 reaches 1.35; over a cache of bf16 k_gqa_prefill
+// takes 530); 509 tokens behind 20011 of 12 heads on 3 with two maps of 64 / 128 149 us (0.64), 130 tokens of 12 heads 12.5.  Phases one behind the other, two groups of four waves: 515,
 // 226, 11.5.
 // One barrier a tile: what is read and written between two of them is in kv8_schedule.hpp.
 // Wave 0 makes the values' factors a tile ahead, wave 1 the keys' scales two.  A value without a scale takes its key's away instead, so that only queries that see it lose theirs.

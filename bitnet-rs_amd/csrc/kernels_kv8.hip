@@ -1258,7 +1258,8 @@ __global__ __launch_bounds__(64 * W * G, NV > 8 || NK > 2 || (NK == 2 && MAPS ==
 static bool maps_apart(const Gqa &g) { return g.maps == 2 && (g.dimp > 128 || g.vdimp > 128); }
 bool kv8_prefill_wants_records(const Gqa &g) { return maps_apart(g); }
 
-// Waves that share a tile, groups of them that share the rows, and stretches of the keys.  us of a step of a walk (128 columns): four waves 1.72, with two such workgroups on a compute unit
+// Waves that share a tile, groups of them that share the rows, and stretches of the keys.  us of a step of a walk that the rule counts with (128 columns; measured last 1.77, 2.5, 2.15 for 1.72, 2.44, 1.98, which
+// chooses no better: over eight shapes and eight lengths the forms taken are 2 % above the best on average, 20 % at most): four waves 1.72, with two such workgroups on a compute unit
 // 2.4; two groups of four waves 2.44 for two tiles; eight waves (twice the rows) 1.98; heads of more than 128 columns 3.3, one workgroup on a compute unit; two maps of 65 to 128 columns 2.4
 // whatever the waves, one workgroup.  A launch lasts as long as its longest walk, or as its share of all of them with what workgroups of unequal length leave idle (an eighth; more where few
 // long ones share a compute unit's time).  Records cost 5 us and their bytes, 0.23 ns for 132 floats.
